@@ -16,12 +16,12 @@
 // D(r+1,c+1) of one pair is D(r,c) of the next, so each pair costs ONE distance.  A lane owns 8
 // adjacent diagonals as two "streams" A and B of 4 and walks rows in macro steps of 4 (32 pairs,
 // 32 sqrt); two macro steps make a TILE of 8 rows x 8 diagonals.  Every value of a step is an
-// (A, B) register pair, so the subtractions, squares and sums issue as v_pk_add/v_pk_mul/v_pk_fma_f32
-// (measured on MI355X: 25 SIMD-cycles per 64 pairs against 37 for the scalar form,
-// tools/valu_chain_microbench.hip).  Tour-ordered, centred and scaled fp32 coordinates sit in LDS as
+// (A, B) register pair; the build keeps the compiler from packing them (v_pk_add/mul/fma_f32 would take 25
+// SIMD-cycles per 64 pairs against 37 for the scalar form, tools/valu_chain_microbench.hip, but have given
+// wrong results now and then), which costs the TSP-500 x 2048 batch 15.1 -> 17.4 ms.  Tour-ordered, centred and scaled fp32 coordinates sit in LDS as
 // three 8-way interleaved arrays (x, y, edge length) whose entries are already the (A, B) pairs
 // (value at window position w and at w + 4), so one conflict-free ds_read_b64 per operand feeds the
-// packed math with no register moves; row operands are broadcast reads of the same arrays.
+// math with no register moves; row operands are broadcast reads of the same arrays.
 //
 // The fp32 value is only a FILTER with a proven error bound eps: every lane keeps its best tile a1
 // and runner-up a2; after a workgroup min m only tiles with a1 <= m + 2 eps can hold the true argmin.
