@@ -25,6 +25,8 @@ extern "C" {
 
 #define TSP2OPT_DTYPE_F32 0            /* arithmetic in float, like the plugin with fp32 points */
 #define TSP2OPT_DTYPE_F64 1            /* arithmetic in double, like tsp_2opt (two_opt.py:67)   */
+#define TSP2OPT_DTYPE_BF16 2           /* storage of the learning operators below (float arithmetic) */
+#define TSP2OPT_DTYPE_F16 3            /* same                                                       */
 
 /* return codes */
 #define TSP2OPT_OK              0
@@ -252,6 +254,79 @@ int tsp2opt_gls_rounds(const double* points, int64_t* tours, int64_t* best_tours
                        int64_t num_tours, int32_t n, int32_t tours_per_instance, int32_t tours_per_map,
                        int32_t perturbation_moves, int32_t rounds, int32_t init, int32_t device,
                        void* hip_stream);
+
+/*
+ * Learning operators: from tours back to the heat map (or the autoregressive decoder) they were drawn from.
+ * No counterpart in the reference's native code; its trainers do this with chains of torch kernels per decoding step.
+ * All of them only enqueue kernels on `hip_stream` (no allocation, no memset, no host synchronisation; they may be
+ * captured), use no atomics, add in a fixed order (bit-identical from run to run) and compute in float with double
+ * sums over steps; `dtype` (TSP2OPT_DTYPE_F32, _BF16 or _F16) is only how an array is stored.  `state` is device memory
+ * of the caller, 256-byte aligned, written by the forward call and read by its gradient call.
+ *
+ * tsp2opt_tour_logprobs -- step log-probabilities of tours (sampling procedure ml4tsp/nar/decoder/sampling.py:21-43 on
+ * the heat map exp(logits)): step s = 0 .. n-2 of tour t chooses t[s+1] among the nodes not visited yet with the
+ * softmax of a row of logits.
+ *   logits   (num_tours / tours_per_map, n, n) with rows = 0: row = the node t[s] that is left;
+ *            (num_tours, n - 1, n) with rows = 1 (tours_per_map = 1): row = the step s.
+ *            map_stride / row_stride in elements, elements of a row adjacent
+ *   tours    (num_tours, n+1) int64 (the last entry is not read: closing a tour is no choice)
+ *   logp_out (num_tours, n-1) float
+ * Entries of visited nodes (the diagonal among them) are never used, whatever they hold.  A step whose open entries
+ * are all -inf gets -inf, a chosen -inf among finite ones too; NaN or +inf among the open entries gives NaN.  A tour
+ * that is no permutation of 0 .. n-1 gets NaN in all its steps and adds nothing to the gradient.
+ * tsp2opt_tour_logprobs_grad -- grad_out (same shape as logits, contiguous, same dtype) from grad_logp
+ * (num_tours, n-1) float.  A step whose grad_logp is 0, or whose open entries are all -inf, adds nothing.
+ */
+int64_t tsp2opt_tour_logprobs_state_bytes(int64_t num_tours, int32_t n, int32_t tours_per_map, int32_t rows);
+int tsp2opt_tour_logprobs(const void* logits, const int64_t* tours, float* logp_out, void* state,
+                          int64_t state_bytes, int64_t num_tours, int32_t n, int32_t tours_per_map, int32_t rows,
+                          int64_t map_stride, int64_t row_stride, int32_t dtype, int32_t device, void* hip_stream);
+int tsp2opt_tour_logprobs_grad(const void* logits, const int64_t* tours, const void* state, int64_t state_bytes,
+                               const float* grad_logp, void* grad_out, int64_t num_tours, int32_t n,
+                               int32_t tours_per_map, int32_t rows, int64_t map_stride, int64_t row_stride,
+                               int32_t dtype, int32_t device, void* hip_stream);
+
+/*
+ * tsp2opt_policy_loss -- clipped policy loss with a KL term on step log-probabilities (num_tours, steps):
+ *   x = logp - old_logp (ratio_of_tour: summed over the tour's kept steps), r = exp x,
+ *   term = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(d) - 1 - d with d = ref_logp - logp per step,
+ *   loss = average(term) + kl_coef * average(kl)
+ *   average_of_tours 0: over all kept steps; 1: over a tour's kept steps, then over the tours that have any
+ *   ref_logp  NULL: no KL term (kl_coef must be 0);  advantages (num_tours) or, adv_per_step, (num_tours, steps) float
+ *   mask      (num_tours, steps) bytes, 0 = step does not count and its values are not used; NULL: all count
+ *   loss_out  1 float; stats_out 2 floats: average kl, share of clipped steps (tours).  Nothing kept: all 0
+ * tsp2opt_policy_loss_grad -- grad_out (num_tours, steps) in `dtype` = grad_loss[0] * d loss / d logp, 0 at steps that
+ * do not count.  Where the clipped branch is the smaller one the ratio's gradient is 0; the side is decided in double.
+ */
+int64_t tsp2opt_policy_loss_state_bytes(int64_t num_tours);
+int tsp2opt_policy_loss(const void* logp, const void* old_logp, const void* ref_logp, const float* advantages,
+                        const uint8_t* mask, float* loss_out, float* stats_out, void* state, int64_t state_bytes,
+                        int64_t num_tours, int64_t steps, int32_t adv_per_step, int32_t ratio_of_tour,
+                        int32_t average_of_tours, double clip_low, double clip_high, double kl_coef, int32_t dtype,
+                        int32_t device, void* hip_stream);
+int tsp2opt_policy_loss_grad(const void* logp, const void* old_logp, const void* ref_logp, const float* advantages,
+                             const uint8_t* mask, const void* state, int64_t state_bytes, const float* grad_loss,
+                             void* grad_out, int64_t num_tours, int64_t steps, int32_t adv_per_step,
+                             int32_t ratio_of_tour, int32_t average_of_tours, double clip_low, double clip_high,
+                             double kl_coef, int32_t dtype, int32_t device, void* hip_stream);
+
+/*
+ * tsp2opt_preference_loss -- preference loss over the tours of every instance, the shorter tour preferred:
+ *   s = beta * sum over kept steps of (logp - ref_logp) (per_step: their mean), and over all pairs (a, b) of tours of
+ *   one instance with lengths[a] < lengths[b] (best_only: a = the instance's first shortest tour only) the average of
+ *   -(1 - label_smoothing) log sigmoid(s_a - s_b) - label_smoothing log sigmoid(s_b - s_a)
+ *   lengths   (num_tours) double, as tsp2opt_evaluate writes them; equal lengths are no pair, NaN is in none
+ *   ref_logp, mask  as above, or NULL;  loss_out 1 float, pairs_out 1 int64.  No pair: loss 0
+ * tsp2opt_preference_loss_grad -- grad_out (num_tours, steps) in `dtype` = grad_loss[0] * d loss / d logp.
+ */
+int64_t tsp2opt_preference_loss_state_bytes(int64_t num_tours);
+int tsp2opt_preference_loss(const void* logp, const void* ref_logp, const double* lengths, const uint8_t* mask,
+                            float* loss_out, int64_t* pairs_out, void* state, int64_t state_bytes, int64_t num_tours,
+                            int64_t steps, int32_t tours_per_instance, int32_t best_only, int32_t per_step,
+                            double beta, double label_smoothing, int32_t dtype, int32_t device, void* hip_stream);
+int tsp2opt_preference_loss_grad(const uint8_t* mask, const void* state, int64_t state_bytes, const float* grad_loss,
+                                 void* grad_out, int64_t num_tours, int64_t steps, int32_t dtype, int32_t device,
+                                 void* hip_stream);
 
 /*
  * tsp2opt_sqrt_check -- numerics self-test used by the GPU test-suite: out[k] = sqrt(in[k])

@@ -17,6 +17,9 @@ from .local_search import (  # noqa: F401
 from .local_ops import (  # noqa: F401,E402
     tsp_relocate, tsp_ls, tsp_gls, ML4TSPNARGuidedLS, ls_step_device, local_search_device, guided_ls_device,
 )
+from .learning import (  # noqa: F401,E402
+    tour_log_probs, clipped_policy_loss, preference_loss, PolicyLossResult, PreferenceLossResult,
+)
 from .anytime import two_opt_anytime, AnytimeResult  # noqa: F401,E402
 
 # the legacy registry's other local searches (search/__init__.py:45-52)
@@ -25,6 +28,7 @@ LOCAL_SEARCH_CLASS[("tsp", "ls")] = tsp_ls
 LOCAL_SEARCH_CLASS[("tsp", "gls")] = tsp_gls
 
 __all__ = [
+    "tour_log_probs", "clipped_policy_loss", "preference_loss", "PolicyLossResult", "PreferenceLossResult",
     "two_opt_anytime", "AnytimeResult",
     "tsp_relocate", "tsp_ls", "tsp_gls", "ML4TSPNARGuidedLS", "ls_step_device", "local_search_device", "guided_ls_device",
     "batched_two_opt_torch", "tsp_2opt", "two_opt_device", "TwoOptResult", "evaluate_tours", "EvalResult",

@@ -15,6 +15,8 @@ LIB_PATH = os.environ.get("TSP2OPT_LIB") or os.path.join(_HERE, "libtsp2opt_hip.
 
 DTYPE_F32 = 0
 DTYPE_F64 = 1
+DTYPE_BF16 = 2
+DTYPE_F16 = 3
 
 ST_BAD_INDEX = 1
 ST_NOT_CLOSED = 2
@@ -44,6 +46,15 @@ SYMBOLS = (
     "tsp2opt_ls_step",
     "tsp2opt_local_search",
     "tsp2opt_gls_rounds",
+    "tsp2opt_tour_logprobs_state_bytes",
+    "tsp2opt_tour_logprobs",
+    "tsp2opt_tour_logprobs_grad",
+    "tsp2opt_policy_loss_state_bytes",
+    "tsp2opt_policy_loss",
+    "tsp2opt_policy_loss_grad",
+    "tsp2opt_preference_loss_state_bytes",
+    "tsp2opt_preference_loss",
+    "tsp2opt_preference_loss_grad",
     "tsp2opt_sqrt_check",
     "tsp2opt_plan",
     "tsp2opt_debug_greedy_cycles",
@@ -113,6 +124,27 @@ def lib() -> ctypes.CDLL:
     L.tsp2opt_greedy_decode_sparse.restype = ctypes.c_int
     L.tsp2opt_greedy_sparse_workspace_bytes.argtypes = [i64, i32, i64, i32, i32]
     L.tsp2opt_greedy_sparse_workspace_bytes.restype = i64
+    L.tsp2opt_tour_logprobs_state_bytes.argtypes = [i64, i32, i32, i32]
+    L.tsp2opt_tour_logprobs_state_bytes.restype = i64
+    L.tsp2opt_tour_logprobs.argtypes = [vp, vp, vp, vp, i64, i64, i32, i32, i32, i64, i64, i32, i32, vp]
+    L.tsp2opt_tour_logprobs.restype = ctypes.c_int
+    L.tsp2opt_tour_logprobs_grad.argtypes = [vp, vp, vp, i64, vp, vp, i64, i32, i32, i32, i64, i64, i32, i32, vp]
+    L.tsp2opt_tour_logprobs_grad.restype = ctypes.c_int
+    L.tsp2opt_policy_loss_state_bytes.argtypes = [i64]
+    L.tsp2opt_policy_loss_state_bytes.restype = i64
+    L.tsp2opt_policy_loss.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, i32, i32, f64, f64, f64,
+                                      i32, i32, vp]
+    L.tsp2opt_policy_loss.restype = ctypes.c_int
+    L.tsp2opt_policy_loss_grad.argtypes = [vp, vp, vp, vp, vp, vp, i64, vp, vp, i64, i64, i32, i32, i32, f64, f64, f64,
+                                           i32, i32, vp]
+    L.tsp2opt_policy_loss_grad.restype = ctypes.c_int
+    L.tsp2opt_preference_loss_state_bytes.argtypes = [i64]
+    L.tsp2opt_preference_loss_state_bytes.restype = i64
+    L.tsp2opt_preference_loss.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, i32, i32, f64, f64, i32, i32,
+                                          vp]
+    L.tsp2opt_preference_loss.restype = ctypes.c_int
+    L.tsp2opt_preference_loss_grad.argtypes = [vp, vp, i64, vp, vp, i64, i64, i32, i32, vp]
+    L.tsp2opt_preference_loss_grad.restype = ctypes.c_int
     L.tsp2opt_sqrt_check.argtypes = [vp, vp, i64, i32, i32, vp]
     L.tsp2opt_sqrt_check.restype = ctypes.c_int
     L.tsp2opt_plan.argtypes = [i32, i32, i32, ctypes.POINTER(i32)]

@@ -13,9 +13,11 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SRCS = [os.path.join(HERE, "csrc", f) for f in ("tsp2opt.hip", "greedy.hip", "greedy_sparse.hip", "ls_ops.hip")]
+SRCS = [os.path.join(HERE, "csrc", f) for f in ("tsp2opt.hip", "greedy.hip", "greedy_sparse.hip", "ls_ops.hip",
+                                                "tour_logprobs.hip", "policy_loss.hip")]
 DEPS = [os.path.join(HERE, "csrc", f) for f in ("wave_reduce.hpp", "host_util.hpp", "two_opt_common.hpp",
-                                                 "two_opt_kernel.hpp", "two_opt_band.hpp", "two_opt_aux.hpp")]
+                                                 "two_opt_kernel.hpp", "two_opt_band.hpp", "two_opt_aux.hpp",
+                                                 "learn_common.hpp")]
 HDR = os.path.join(ROOT, "include", "tsp2opt.h")
 LIB = os.path.join(HERE, "libtsp2opt_hip.so")
 
@@ -36,6 +38,8 @@ UNIT_DEPS = {
     "greedy.hip": ("wave_reduce.hpp", "host_util.hpp", "greedy_walk.hpp"),
     "greedy_sparse.hip": ("wave_reduce.hpp", "host_util.hpp", "greedy_walk.hpp"),
     "ls_ops.hip": ("wave_reduce.hpp", "host_util.hpp"),
+    "tour_logprobs.hip": ("learn_common.hpp", "host_util.hpp"),
+    "policy_loss.hip": ("learn_common.hpp", "host_util.hpp"),
 }
 
 

@@ -1,0 +1,298 @@
+"""From tours back to the heat map: log-probabilities of tours and the losses that turn lengths into a gradient.
+
+What ``greedy_decode_device`` / a sampling decoder (``ml4tsp/nar/decoder/sampling.py:21-43``) draws from a heat map,
+``two_opt_device`` improves and ``evaluate_tours`` measures is scored here under the heat map (or under the logits that
+an autoregressive decoder wrote), with gradients for ``torch.autograd``: ``tour_log_probs`` (csrc/tour_logprobs.hip),
+``clipped_policy_loss`` and ``preference_loss`` (csrc/policy_loss.hip).
+
+Everything runs on the current stream of the tensors' device, without host synchronisation, and may be captured into a
+graph; results do not change from run to run.  There is no CPU path.  Second derivatives are not available.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_ROWS = {"node": 0, "step": 1}
+
+
+def _code(x: torch.Tensor, name: str) -> int:
+    try:
+        return _CODES[x.dtype]
+    except KeyError:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}") from None
+
+
+def _same_device(first: torch.Tensor, what: str, *others: Optional[torch.Tensor]) -> torch.device:
+    if first.device.type != "cuda" or any(o is not None and o.device != first.device for o in others):
+        raise ValueError(f"{what} must live on the same HIP device")
+    return first.device
+
+
+def _ptr(x: Optional[torch.Tensor]):
+    return None if x is None else x.data_ptr()
+
+
+def _state(dev: torch.device, nbytes: int, what: str) -> torch.Tensor:
+    """Device memory between a call and its gradient call: one allocation a call, so that calls on other streams and
+    captured graphs never share it."""
+    _lib.check(nbytes, what)
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+class _TourLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tours, per, rows):
+        dev = logits.device
+        T, n = tours.shape[0], tours.shape[1] - 1
+        code = _CODES[logits.dtype]
+        if logits.stride(2) != 1 and n > 1:
+            logits = logits.contiguous()
+        L = _lib.lib()
+        state = _state(dev, L.tsp2opt_tour_logprobs_state_bytes(T, n, per, rows), "tsp2opt_tour_logprobs_state_bytes")
+        out = torch.empty((T, n - 1), dtype=torch.float32, device=dev)
+        rc = L.tsp2opt_tour_logprobs(logits.data_ptr(), tours.data_ptr(), out.data_ptr(), state.data_ptr(),
+                                     state.numel(), T, n, per, rows, logits.stride(0), logits.stride(1), code,
+                                     dev.index, _stream(dev))
+        _lib.check(rc, "tsp2opt_tour_logprobs")
+        ctx.save_for_backward(logits, tours, state)
+        ctx.how = (per, rows)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, tours, state = ctx.saved_tensors
+        per, rows = ctx.how
+        dev = logits.device
+        T, n = tours.shape[0], tours.shape[1] - 1
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        if n == 1:
+            return grad.zero_(), None, None, None
+        g = g.to(torch.float32).contiguous()
+        L = _lib.lib()
+        rc = L.tsp2opt_tour_logprobs_grad(logits.data_ptr(), tours.data_ptr(), state.data_ptr(), state.numel(),
+                                          g.data_ptr(), grad.data_ptr(), T, n, per, rows, logits.stride(0),
+                                          logits.stride(1), _CODES[logits.dtype], dev.index, _stream(dev))
+        _lib.check(rc, "tsp2opt_tour_logprobs_grad")
+        return grad, None, None, None
+
+
+def tour_log_probs(logits: torch.Tensor, tours: torch.Tensor, *, tours_per_map: int = 1,
+                   rows: str = "node") -> torch.Tensor:
+    """Log-probability of every choice of every tour; differentiable in ``logits``.
+
+    Step ``t = 0 .. N-2`` of a tour chooses ``tours[:, t+1]`` among the nodes it has not visited yet, with the softmax
+    of one row of logits over those nodes.  ``logits`` float32 / bfloat16 / float16:
+
+    * ``rows="node"``: heat maps (M, N, N), the row of the node that is left; tours (M * tours_per_map, N+1), tour ``k``
+      uses map ``k // tours_per_map``.  For a heat map of positive weights pass its logarithm.
+    * ``rows="step"``: what an autoregressive decoder wrote, (T, N-1, N), a row for every step; ``tours_per_map`` is 1.
+
+    Returns (T, N-1) float32; ``.sum(1)`` is a tour's log-likelihood.  Entries of visited nodes are never used, so no
+    mask is needed; -inf (or the type's lowest value) marks forbidden edges.  A step without any open finite entry gets
+    -inf and no gradient, a tour that is no permutation of ``0 .. N-1`` gets NaN and no gradient, and a step whose
+    incoming gradient is 0 contributes nothing.  Asynchronous on the current stream."""
+    if logits.dim() == 2 and rows == "node":
+        return tour_log_probs(logits.unsqueeze(0), tours, tours_per_map=tours_per_map, rows=rows)
+    if tours.dim() == 1:
+        tours = tours.unsqueeze(0)
+    if rows not in _ROWS:
+        raise ValueError(f"rows must be 'node' or 'step', got {rows!r}")
+    _code(logits, "logits")
+    if tours.dtype.is_floating_point or tours.dtype.is_complex or tours.dtype == torch.bool:
+        raise TypeError(f"tours must be integers, got {tours.dtype}")
+    per = int(tours_per_map)
+    if logits.dim() != 3 or tours.dim() != 2 or per < 1 or tours.shape[1] < 2:
+        raise ValueError("expected logits (M, N, N) or (T, N-1, N) and tours (T, N+1)")
+    T, n = tours.shape[0], tours.shape[1] - 1
+    if rows == "step" and per != 1:
+        raise ValueError("rows='step' has logits of its own for every tour: tours_per_map must be 1")
+    want = (T // per, n, n) if rows == "node" else (T, n - 1, n)
+    if tuple(logits.shape) != want or T % per:
+        raise ValueError(f"expected logits {want} for {T} tours of {n} nodes, {per} a map, got {tuple(logits.shape)}")
+    _same_device(logits, "logits and tours", tours)
+    return _TourLogProbs.apply(logits, tours.to(torch.int64).contiguous(), per, _ROWS[rows])
+
+
+@dataclass
+class PolicyLossResult:
+    """Device-resident result of ``clipped_policy_loss``."""
+    loss: torch.Tensor              # () float32, differentiable in log_probs
+    kl: torch.Tensor                # () float32 average of exp(d) - 1 - d (not multiplied by kl_coef)
+    clip_fraction: torch.Tensor     # () float32 share of the steps (tours) whose ratio is clipped
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lp, old, ref, adv, mask, how):
+        dev = lp.device
+        T, S = lp.shape
+        lp, old = lp.contiguous(), old.contiguous()
+        L = _lib.lib()
+        state = _state(dev, L.tsp2opt_policy_loss_state_bytes(T), "tsp2opt_policy_loss_state_bytes")
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        stats = torch.empty(2, dtype=torch.float32, device=dev)
+        rc = L.tsp2opt_policy_loss(lp.data_ptr(), old.data_ptr(), _ptr(ref), adv.data_ptr(), _ptr(mask),
+                                   loss.data_ptr(), stats.data_ptr(), state.data_ptr(), state.numel(), T, S,
+                                   int(adv.dim() == 2), *how, _CODES[lp.dtype], dev.index, _stream(dev))
+        _lib.check(rc, "tsp2opt_policy_loss")
+        ctx.save_for_backward(lp, old, ref, adv, mask, state)
+        ctx.how = how
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        lp, old, ref, adv, mask, state = ctx.saved_tensors
+        dev = lp.device
+        T, S = lp.shape
+        grad = torch.empty_like(lp)
+        g = g.to(torch.float32)
+        rc = _lib.lib().tsp2opt_policy_loss_grad(
+            lp.data_ptr(), old.data_ptr(), _ptr(ref), adv.data_ptr(), _ptr(mask), state.data_ptr(), state.numel(),
+            g.data_ptr(), grad.data_ptr(), T, S, int(adv.dim() == 2), *ctx.how, _CODES[lp.dtype], dev.index,
+            _stream(dev))
+        _lib.check(rc, "tsp2opt_policy_loss_grad")
+        return grad, None, None, None, None, None
+
+
+def _step_arrays(log_probs, mask, **others):
+    """Checks shared by the losses: (T, S) arrays of one type, a boolean mask."""
+    _code(log_probs, "log_probs")
+    if log_probs.dim() != 2:
+        raise ValueError("expected log_probs (T, steps)")
+    for name, x in others.items():
+        if x is None:
+            continue
+        if x.dtype != log_probs.dtype:
+            raise TypeError(f"{name} must have the type of log_probs, {log_probs.dtype}, got {x.dtype}")
+        if x.shape != log_probs.shape:
+            raise ValueError(f"{name} must have the shape of log_probs, {tuple(log_probs.shape)}, got {tuple(x.shape)}")
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise TypeError(f"mask must be boolean, got {mask.dtype}")
+        if mask.shape != log_probs.shape:
+            raise ValueError(f"mask must have the shape of log_probs, {tuple(log_probs.shape)}, got {tuple(mask.shape)}")
+
+
+def clipped_policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor, *,
+                        ref_log_probs: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                        clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, ratio: str = "step",
+                        average: Optional[str] = None) -> PolicyLossResult:
+    """Clipped policy loss with a KL term; differentiable in ``log_probs``.
+
+    ``log_probs`` / ``old_log_probs`` / ``ref_log_probs`` (T, S) of one type (float32, bfloat16, float16): the steps of
+    ``tour_log_probs`` now, when the tours were drawn, and under a reference.  ``advantages`` (T,) or (T, S).
+    ``mask`` (T, S) boolean, True where a step counts (the others' values are not used).
+
+    ``-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)`` with ``r = exp(log_probs - old_log_probs)`` for every step,
+    or with ``ratio="tour"`` of the tour's summed difference (advantages (T,)), plus ``kl_coef`` times
+    ``exp(d) - 1 - d``, ``d = ref_log_probs - log_probs`` of every step.  ``average="step"`` (the default for ratios of
+    steps): over all steps that count; ``"tour"`` (always for ratios of tours): over a tour's steps, then over the tours
+    that have any.  Nothing that counts: loss 0.  Asynchronous on the current stream."""
+    _step_arrays(log_probs, mask, old_log_probs=old_log_probs, ref_log_probs=ref_log_probs)
+    if ratio not in ("step", "tour") or average not in (None, "step", "tour"):
+        raise ValueError("ratio and average must be 'step' or 'tour'")
+    average = average or ratio
+    if ratio == "tour" and average != "tour":
+        raise ValueError("ratios of tours are averaged over tours")
+    T, S = log_probs.shape
+    if tuple(advantages.shape) not in ((T,), (T, S)) or (ratio == "tour" and advantages.dim() != 1):
+        raise ValueError("advantages must be (T,), or (T, steps) with ratios of steps")
+    if not advantages.dtype.is_floating_point:
+        raise TypeError(f"advantages must be floating point, got {advantages.dtype}")
+    if not (0.0 <= clip_low < 1.0 and clip_high >= 0.0 and kl_coef >= 0.0):
+        raise ValueError("clip_low must be in [0, 1), clip_high and kl_coef >= 0")
+    if kl_coef and ref_log_probs is None:
+        raise ValueError("kl_coef needs ref_log_probs")
+    _same_device(log_probs, "log_probs and the other arrays", old_log_probs, advantages, ref_log_probs, mask)
+    how = (int(ratio == "tour"), int(average == "tour"), float(clip_low), float(clip_high), float(kl_coef))
+    ref = None if ref_log_probs is None else ref_log_probs.detach().contiguous()
+    loss, stats = _PolicyLoss.apply(log_probs, old_log_probs.detach(), ref,
+                                    advantages.detach().to(torch.float32).contiguous(),
+                                    None if mask is None else mask.contiguous(), how)
+    return PolicyLossResult(loss, stats[0], stats[1])
+
+
+@dataclass
+class PreferenceLossResult:
+    """Device-resident result of ``preference_loss``."""
+    loss: torch.Tensor              # () float32, differentiable in log_probs
+    num_pairs: torch.Tensor         # () int64 pairs the loss is the average of
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, lp, ref, lengths, mask, how):
+        dev = lp.device
+        T, S = lp.shape
+        lp = lp.contiguous()
+        L = _lib.lib()
+        state = _state(dev, L.tsp2opt_preference_loss_state_bytes(T), "tsp2opt_preference_loss_state_bytes")
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        pairs = torch.empty((), dtype=torch.int64, device=dev)
+        rc = L.tsp2opt_preference_loss(lp.data_ptr(), _ptr(ref), lengths.data_ptr(), _ptr(mask), loss.data_ptr(),
+                                       pairs.data_ptr(), state.data_ptr(), state.numel(), T, S, *how,
+                                       _CODES[lp.dtype], dev.index, _stream(dev))
+        _lib.check(rc, "tsp2opt_preference_loss")
+        ctx.save_for_backward(mask, state)
+        ctx.like = (lp.shape, lp.dtype)
+        ctx.mark_non_differentiable(pairs)
+        return loss, pairs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _):
+        mask, state = ctx.saved_tensors
+        (T, S), dtype = ctx.like
+        dev = state.device
+        grad = torch.empty((T, S), dtype=dtype, device=dev)
+        g = g.to(torch.float32)
+        rc = _lib.lib().tsp2opt_preference_loss_grad(_ptr(mask), state.data_ptr(), state.numel(), g.data_ptr(),
+                                                     grad.data_ptr(), T, S, _CODES[dtype], dev.index, _stream(dev))
+        _lib.check(rc, "tsp2opt_preference_loss_grad")
+        return grad, None, None, None, None
+
+
+def preference_loss(log_probs: torch.Tensor, lengths: torch.Tensor, *, tours_per_instance: int,
+                    ref_log_probs: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                    beta: float = 1.0, label_smoothing: float = 0.0, pairs: str = "all",
+                    per_step: bool = False) -> PreferenceLossResult:
+    """Preference loss over the tours of every instance, the shorter one preferred; differentiable in ``log_probs``.
+
+    ``log_probs`` / ``ref_log_probs`` (T, S) of one type, T = I * tours_per_instance; ``lengths`` (T,) as
+    ``evaluate_tours`` gives them; ``mask`` as in ``clipped_policy_loss``.  A tour's score is ``beta`` times the sum
+    (``per_step``: mean) over its steps of ``log_probs - ref_log_probs``; over all pairs of tours of one instance whose
+    lengths differ (``pairs="best"``: only those with the instance's first shortest tour) the loss is the average of
+    ``-(1 - label_smoothing) log sigmoid(s_short - s_long) - label_smoothing log sigmoid(s_long - s_short)``.
+    Sampled tours against the same tours after ``two_opt_device``: stack them as an instance's tours.  NaN lengths are
+    in no pair; without any pair the loss is 0.  Asynchronous on the current stream."""
+    _step_arrays(log_probs, mask, ref_log_probs=ref_log_probs)
+    per = int(tours_per_instance)
+    T = log_probs.shape[0]
+    if per < 1 or T % per or tuple(lengths.shape) != (T,):
+        raise ValueError("expected log_probs (I * tours_per_instance, steps) and lengths (I * tours_per_instance,)")
+    if lengths.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"lengths must be float32 or float64, got {lengths.dtype}")
+    if pairs not in ("all", "best"):
+        raise ValueError(f"pairs must be 'all' or 'best', got {pairs!r}")
+    if not (beta > 0.0 and 0.0 <= label_smoothing < 0.5):
+        raise ValueError("beta must be > 0 and label_smoothing in [0, 0.5)")
+    _same_device(log_probs, "log_probs and the other arrays", lengths, ref_log_probs, mask)
+    how = (per, int(pairs == "best"), int(bool(per_step)), float(beta), float(label_smoothing))
+    loss, count = _PreferenceLoss.apply(log_probs, None if ref_log_probs is None else ref_log_probs.detach().contiguous(),
+                                        lengths.detach().to(torch.float64).contiguous(),
+                                        None if mask is None else mask.contiguous(), how)
+    return PreferenceLossResult(loss, count)
