@@ -175,6 +175,29 @@ def lib() -> ctypes.CDLL:
     return L
 
 
+_learning_ext = None
+
+# the entry points that the autograd nodes of the learning operators call, in the order of their bind()
+_LEARNING = ("last_error", "tour_logprobs_state_bytes", "tour_logprobs", "tour_logprobs_grad",
+             "policy_loss_state_bytes", "policy_loss", "policy_loss_grad", "preference_loss_state_bytes",
+             "preference_loss", "preference_loss_grad")
+
+
+def learning_ext():
+    """The autograd nodes of the learning operators, bound to the library that lib() loaded."""
+    global _learning_ext
+    if _learning_ext is None:
+        L = lib()
+        try:
+            from . import _learning_ext as ext
+        except ImportError as e:
+            raise Tsp2optError(f"_learning_ext.so is missing or does not load ({e}): build it with "
+                               "`python -m ml4tspbench_amd.build`. There is no fallback.") from None
+        ext.bind([ctypes.cast(getattr(L, "tsp2opt_" + f), ctypes.c_void_p).value for f in _LEARNING], Tsp2optError)
+        _learning_ext = ext
+    return _learning_ext
+
+
 def check(rc: int, what: str) -> None:
     if rc < 0:
         msg = lib().tsp2opt_last_error()

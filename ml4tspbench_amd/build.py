@@ -43,6 +43,31 @@ UNIT_DEPS = {
 }
 
 
+EXT_SRC = os.path.join(HERE, "csrc", "learning_ext.cpp")
+EXT = os.path.join(HERE, "_learning_ext.so")
+
+
+def build_learning_ext(force: bool = False, verbose: bool = False) -> str:
+    """_learning_ext.so: autograd nodes over the C ABI (host code, g++ against the installed torch)."""
+    if not force and os.path.exists(EXT) and os.path.getmtime(EXT) >= max(os.path.getmtime(f) for f in (EXT_SRC, HDR, __file__)):
+        return EXT
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(HIPCC))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_learning_ext",
+           "-I", os.path.join(ROOT, "include"), "-isystem", os.path.join(root, "include"),
+           "-isystem", os.path.join(rocm, "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-o", EXT, EXT_SRC, "-L", os.path.join(root, "lib"),
+           "-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lc10_hip", "-ltorch_hip"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return EXT
+
+
 def build(force: bool = False, verbose: bool = False, fine: bool = False) -> str:
     """fine=True: the diagnostic variant libtsp2opt_hip_fine.so (-DTSP2OPT_FINE: sub-phase cycle marks,
     tools/phase_breakdown.py --fine); never the library that is benchmarked or shipped."""
@@ -79,4 +104,5 @@ def build(force: bool = False, verbose: bool = False, fine: bool = False) -> str
 
 
 if __name__ == "__main__":
+    print(build_learning_ext(force="--force" in sys.argv, verbose=True))
     print(build(force="--force" in sys.argv, verbose=True, fine="--fine" in sys.argv))

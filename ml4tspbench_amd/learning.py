@@ -6,7 +6,8 @@ an autoregressive decoder wrote), with gradients for ``torch.autograd``: ``tour_
 ``clipped_policy_loss`` and ``preference_loss`` (csrc/policy_loss.hip).
 
 Everything runs on the current stream of the tensors' device, without host synchronisation, and may be captured into a
-graph; results do not change from run to run.  There is no CPU path.  Second derivatives are not available.
+graph; results do not change from run to run.  There is no CPU path, and no second derivative.  The autograd nodes are
+csrc/learning_ext.cpp.
 """
 from __future__ import annotations
 
@@ -14,78 +15,22 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
-_CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _ROWS = {"node": 0, "step": 1}
 
 
-def _code(x: torch.Tensor, name: str) -> int:
-    try:
-        return _CODES[x.dtype]
-    except KeyError:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}") from None
+def _check_type(x: torch.Tensor, name: str) -> None:
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
 
 
 def _same_device(first: torch.Tensor, what: str, *others: Optional[torch.Tensor]) -> torch.device:
     if first.device.type != "cuda" or any(o is not None and o.device != first.device for o in others):
         raise ValueError(f"{what} must live on the same HIP device")
     return first.device
-
-
-def _ptr(x: Optional[torch.Tensor]):
-    return None if x is None else x.data_ptr()
-
-
-def _state(dev: torch.device, nbytes: int, what: str) -> torch.Tensor:
-    """Device memory between a call and its gradient call: one allocation a call, so that calls on other streams and
-    captured graphs never share it."""
-    _lib.check(nbytes, what)
-    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev)
-
-
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-class _TourLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tours, per, rows):
-        dev = logits.device
-        T, n = tours.shape[0], tours.shape[1] - 1
-        code = _CODES[logits.dtype]
-        if logits.stride(2) != 1 and n > 1:
-            logits = logits.contiguous()
-        L = _lib.lib()
-        state = _state(dev, L.tsp2opt_tour_logprobs_state_bytes(T, n, per, rows), "tsp2opt_tour_logprobs_state_bytes")
-        out = torch.empty((T, n - 1), dtype=torch.float32, device=dev)
-        rc = L.tsp2opt_tour_logprobs(logits.data_ptr(), tours.data_ptr(), out.data_ptr(), state.data_ptr(),
-                                     state.numel(), T, n, per, rows, logits.stride(0), logits.stride(1), code,
-                                     dev.index, _stream(dev))
-        _lib.check(rc, "tsp2opt_tour_logprobs")
-        ctx.save_for_backward(logits, tours, state)
-        ctx.how = (per, rows)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, tours, state = ctx.saved_tensors
-        per, rows = ctx.how
-        dev = logits.device
-        T, n = tours.shape[0], tours.shape[1] - 1
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        if n == 1:
-            return grad.zero_(), None, None, None
-        g = g.to(torch.float32).contiguous()
-        L = _lib.lib()
-        rc = L.tsp2opt_tour_logprobs_grad(logits.data_ptr(), tours.data_ptr(), state.data_ptr(), state.numel(),
-                                          g.data_ptr(), grad.data_ptr(), T, n, per, rows, logits.stride(0),
-                                          logits.stride(1), _CODES[logits.dtype], dev.index, _stream(dev))
-        _lib.check(rc, "tsp2opt_tour_logprobs_grad")
-        return grad, None, None, None
 
 
 def tour_log_probs(logits: torch.Tensor, tours: torch.Tensor, *, tours_per_map: int = 1,
@@ -109,7 +54,7 @@ def tour_log_probs(logits: torch.Tensor, tours: torch.Tensor, *, tours_per_map: 
         tours = tours.unsqueeze(0)
     if rows not in _ROWS:
         raise ValueError(f"rows must be 'node' or 'step', got {rows!r}")
-    _code(logits, "logits")
+    _check_type(logits, "logits")
     if tours.dtype.is_floating_point or tours.dtype.is_complex or tours.dtype == torch.bool:
         raise TypeError(f"tours must be integers, got {tours.dtype}")
     per = int(tours_per_map)
@@ -122,7 +67,7 @@ def tour_log_probs(logits: torch.Tensor, tours: torch.Tensor, *, tours_per_map: 
     if tuple(logits.shape) != want or T % per:
         raise ValueError(f"expected logits {want} for {T} tours of {n} nodes, {per} a map, got {tuple(logits.shape)}")
     _same_device(logits, "logits and tours", tours)
-    return _TourLogProbs.apply(logits, tours.to(torch.int64).contiguous(), per, _ROWS[rows])
+    return _lib.learning_ext().tour_log_probs(logits, tours, per, _ROWS[rows])
 
 
 @dataclass
@@ -133,44 +78,9 @@ class PolicyLossResult:
     clip_fraction: torch.Tensor     # () float32 share of the steps (tours) whose ratio is clipped
 
 
-class _PolicyLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, lp, old, ref, adv, mask, how):
-        dev = lp.device
-        T, S = lp.shape
-        lp, old = lp.contiguous(), old.contiguous()
-        L = _lib.lib()
-        state = _state(dev, L.tsp2opt_policy_loss_state_bytes(T), "tsp2opt_policy_loss_state_bytes")
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        stats = torch.empty(2, dtype=torch.float32, device=dev)
-        rc = L.tsp2opt_policy_loss(lp.data_ptr(), old.data_ptr(), _ptr(ref), adv.data_ptr(), _ptr(mask),
-                                   loss.data_ptr(), stats.data_ptr(), state.data_ptr(), state.numel(), T, S,
-                                   int(adv.dim() == 2), *how, _CODES[lp.dtype], dev.index, _stream(dev))
-        _lib.check(rc, "tsp2opt_policy_loss")
-        ctx.save_for_backward(lp, old, ref, adv, mask, state)
-        ctx.how = how
-        ctx.mark_non_differentiable(stats)
-        return loss, stats
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        lp, old, ref, adv, mask, state = ctx.saved_tensors
-        dev = lp.device
-        T, S = lp.shape
-        grad = torch.empty_like(lp)
-        g = g.to(torch.float32)
-        rc = _lib.lib().tsp2opt_policy_loss_grad(
-            lp.data_ptr(), old.data_ptr(), _ptr(ref), adv.data_ptr(), _ptr(mask), state.data_ptr(), state.numel(),
-            g.data_ptr(), grad.data_ptr(), T, S, int(adv.dim() == 2), *ctx.how, _CODES[lp.dtype], dev.index,
-            _stream(dev))
-        _lib.check(rc, "tsp2opt_policy_loss_grad")
-        return grad, None, None, None, None, None
-
-
 def _step_arrays(log_probs, mask, **others):
     """Checks shared by the losses: (T, S) arrays of one type, a boolean mask."""
-    _code(log_probs, "log_probs")
+    _check_type(log_probs, "log_probs")
     if log_probs.dim() != 2:
         raise ValueError("expected log_probs (T, steps)")
     for name, x in others.items():
@@ -218,12 +128,9 @@ def clipped_policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, ad
     if kl_coef and ref_log_probs is None:
         raise ValueError("kl_coef needs ref_log_probs")
     _same_device(log_probs, "log_probs and the other arrays", old_log_probs, advantages, ref_log_probs, mask)
-    how = (int(ratio == "tour"), int(average == "tour"), float(clip_low), float(clip_high), float(kl_coef))
-    ref = None if ref_log_probs is None else ref_log_probs.detach().contiguous()
-    loss, stats = _PolicyLoss.apply(log_probs, old_log_probs.detach(), ref,
-                                    advantages.detach().to(torch.float32).contiguous(),
-                                    None if mask is None else mask.contiguous(), how)
-    return PolicyLossResult(loss, stats[0], stats[1])
+    return PolicyLossResult(*_lib.learning_ext().policy_loss(
+        log_probs, old_log_probs, ref_log_probs, advantages, mask, ratio == "tour", average == "tour", clip_low, clip_high,
+        kl_coef))
 
 
 @dataclass
@@ -231,39 +138,6 @@ class PreferenceLossResult:
     """Device-resident result of ``preference_loss``."""
     loss: torch.Tensor              # () float32, differentiable in log_probs
     num_pairs: torch.Tensor         # () int64 pairs the loss is the average of
-
-
-class _PreferenceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, lp, ref, lengths, mask, how):
-        dev = lp.device
-        T, S = lp.shape
-        lp = lp.contiguous()
-        L = _lib.lib()
-        state = _state(dev, L.tsp2opt_preference_loss_state_bytes(T), "tsp2opt_preference_loss_state_bytes")
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        pairs = torch.empty((), dtype=torch.int64, device=dev)
-        rc = L.tsp2opt_preference_loss(lp.data_ptr(), _ptr(ref), lengths.data_ptr(), _ptr(mask), loss.data_ptr(),
-                                       pairs.data_ptr(), state.data_ptr(), state.numel(), T, S, *how,
-                                       _CODES[lp.dtype], dev.index, _stream(dev))
-        _lib.check(rc, "tsp2opt_preference_loss")
-        ctx.save_for_backward(mask, state)
-        ctx.like = (lp.shape, lp.dtype)
-        ctx.mark_non_differentiable(pairs)
-        return loss, pairs
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _):
-        mask, state = ctx.saved_tensors
-        (T, S), dtype = ctx.like
-        dev = state.device
-        grad = torch.empty((T, S), dtype=dtype, device=dev)
-        g = g.to(torch.float32)
-        rc = _lib.lib().tsp2opt_preference_loss_grad(_ptr(mask), state.data_ptr(), state.numel(), g.data_ptr(),
-                                                     grad.data_ptr(), T, S, _CODES[dtype], dev.index, _stream(dev))
-        _lib.check(rc, "tsp2opt_preference_loss_grad")
-        return grad, None, None, None, None
 
 
 def preference_loss(log_probs: torch.Tensor, lengths: torch.Tensor, *, tours_per_instance: int,
@@ -291,8 +165,5 @@ def preference_loss(log_probs: torch.Tensor, lengths: torch.Tensor, *, tours_per
     if not (beta > 0.0 and 0.0 <= label_smoothing < 0.5):
         raise ValueError("beta must be > 0 and label_smoothing in [0, 0.5)")
     _same_device(log_probs, "log_probs and the other arrays", lengths, ref_log_probs, mask)
-    how = (per, int(pairs == "best"), int(bool(per_step)), float(beta), float(label_smoothing))
-    loss, count = _PreferenceLoss.apply(log_probs, None if ref_log_probs is None else ref_log_probs.detach().contiguous(),
-                                        lengths.detach().to(torch.float64).contiguous(),
-                                        None if mask is None else mask.contiguous(), how)
-    return PreferenceLossResult(loss, count)
+    return PreferenceLossResult(*_lib.learning_ext().preference_loss(
+        log_probs, ref_log_probs, lengths, mask, per, pairs == "best", bool(per_step), beta, label_smoothing))

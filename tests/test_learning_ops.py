@@ -520,13 +520,13 @@ def test_gpu_policy_loss_edges():
         for shape in ((3, 0), (0, 4)):
             e = torch.zeros(shape, device="cuda", requires_grad=True)
             r = amd.clipped_policy_loss(e, e, torch.zeros(shape[0], device="cuda"), ratio=kind)
-            assert float(r.loss) == 0.0 and torch.autograd.grad(r.loss, e)[0].shape == shape
+            assert float(r.loss.detach()) == 0.0 and torch.autograd.grad(r.loss, e)[0].shape == shape
         res = amd.clipped_policy_loss(lp, lp, adv, ref_log_probs=lp, kl_coef=1.0, ratio=kind)
-        assert float(res.kl) == 0.0 and float(res.loss) == -1.0
+        assert float(res.kl) == 0.0 and float(res.loss.detach()) == -1.0
     x = torch.tensor([[-math.inf, -1.0]], device="cuda", requires_grad=True)      # ruled out since it was drawn: r = 0
     old = torch.tensor([[-2.0, -1.0]], device="cuda")
     res = amd.clipped_policy_loss(x, old, torch.ones(1, device="cuda"))
-    assert float(res.loss) == -0.5 and torch.autograd.grad(res.loss, x)[0].tolist() == [[0.0, -0.5]]
+    assert float(res.loss.detach()) == -0.5 and torch.autograd.grad(res.loss, x)[0].tolist() == [[0.0, -0.5]]
     gen = torch.Generator().manual_seed(12)
     lp, old, ref, adv, mask = policy_inputs(gen, 9, 31, torch.float32, True, True, True)
     wide = torch.zeros((9, 62))
@@ -599,7 +599,7 @@ def test_gpu_preference_loss_edges():
     lp = torch.randn((4, 3), device="cuda", requires_grad=True)
     for length, per in ((torch.ones(4), 4), (torch.arange(4.0), 1), (torch.full((4,), math.nan), 2)):
         res = amd.preference_loss(lp, length.cuda(), tours_per_instance=per)
-        assert float(res.loss) == 0.0 and int(res.num_pairs) == 0
+        assert float(res.loss.detach()) == 0.0 and int(res.num_pairs) == 0
         assert torch.equal(torch.autograd.grad(res.loss, lp)[0], torch.zeros_like(lp))
     a = amd.preference_loss(lp, torch.tensor([1.0, 2, 3, 4]).cuda(), tours_per_instance=2)
     b = amd.preference_loss(lp, torch.tensor([1.0, 2, 3, 4], dtype=torch.float64).cuda(), tours_per_instance=2)
@@ -610,7 +610,7 @@ def test_gpu_preference_loss_edges():
         x = torch.zeros(shape, device="cuda", requires_grad=True)
         res = amd.preference_loss(x, torch.arange(float(shape[0])).cuda(), tours_per_instance=2)
         assert int(res.num_pairs) == (0 if shape[0] == 0 else 2)
-        assert abs(float(res.loss) - (0.0 if shape[0] == 0 else math.log(2))) < 1e-6
+        assert abs(float(res.loss.detach()) - (0.0 if shape[0] == 0 else math.log(2))) < 1e-6
         assert torch.autograd.grad(res.loss, x)[0].shape == shape
 
 
