@@ -13,9 +13,10 @@
 // Several tours a map (k_shared): e_j = exp(h_j - row maximum) does not depend on the tour, only which e_j are added
 // does, and positions are whole numbers, so a masked addition is
 //     S += min(max(pos_j - t, 0), 1) * e_j          (one v_sub with clamp, one v_fmac)
-// instead of an exponential a tour.  That sum loses steps whose open entries all lie far below the row's maximum: below
-// 2^-80 (and where it is NaN) the step is redone alone, relative to its own maximum.  Above it, what float flushes
-// (below 2^-126, 65535 of them at most) is under 2^-30 of the sum.
+// instead of an exponential a tour.  That sum loses steps whose open entries all lie far below the row's maximum, so
+// the exponentials are kept times 2^60, which spends the range of float above 1 too: what it flushes (below 2^-126,
+// 65535 entries at most) is under 2^-30 of a sum above 2^-80, which is 2^-140 = e^-97 relative to the row's maximum.
+// Steps below that (and those that are NaN) are redone alone, relative to their own maximum.
 // One tour a row (k_single): the maximum is the open entries' own, nothing is ever lost.
 #include "learn_common.hpp"
 
@@ -23,7 +24,7 @@ namespace t2o {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kSmall = 0x1p-80f;
+constexpr float kSmall = 0x1p-80f, kScale = 0x1p60f;
 constexpr int kWaves = 8, kRows = 4, kTile = 16;    // k_shared: waves a workgroup, rows a wave, tours a pass
 constexpr int kSingleRows = 16;                     // k_single: rows a wave
 constexpr int kMaxPer = 16;                         // entries of a row a lane holds at most
@@ -54,7 +55,7 @@ __device__ __forceinline__ int64_t work_block()
 
 // Inverse permutation and successors of every tour, one workgroup a tour; scattered in LDS so that the writes are
 // contiguous.
-__global__ __launch_bounds__(256) void k_positions(const int64_t* tours, float* pos, uint16_t* next, float* logp, int n)
+__global__ __launch_bounds__(1024) void k_positions(const int64_t* tours, float* pos, uint16_t* next, float* logp, int n)
 {
     extern __shared__ uint16_t at[];
     const int64_t k = blockIdx.x;
@@ -93,58 +94,86 @@ struct Pack<E, 1> {
     typedef E type;
 };
 
+// Loads are issued without a branch: a lane at or behind the end reads the row's last V entries instead (in front of a
+// short last part there is the previous one) and end_row puts its entries in place.
 template <typename E, int K>
-__device__ __forceinline__ void load_row(const E* row, int lane, int cols, float (&h)[K])
+struct Row {
+    static constexpr int V = kVec<K>;
+    typename Pack<E, V>::type x[K / V];
+};
+
+template <typename E, int K, int G = 64>
+__device__ __forceinline__ void load_row(const E* row, int lane, int cols, Row<E, K>& raw)
 {
     constexpr int V = kVec<K>;
     using P = typename Pack<E, V>::type;
 #pragma unroll
     for (int c = 0; c < K / V; ++c) {
-        const int j = c * 64 * V + lane * V;
-        if ((c + 1) * 64 * V <= cols) {
-            const P x = *reinterpret_cast<const P*>(row + j);
+        const int j = c * G * V + lane * V;
+        raw.x[c] = *reinterpret_cast<const P*>(row + min(j, cols - V));
+    }
+}
+
+template <typename E, int K, int G = 64>
+__device__ __forceinline__ void end_row(const Row<E, K>& raw, int lane, int cols, float (&h)[K])
+{
+    constexpr int V = kVec<K>;
+#pragma unroll
+    for (int c = 0; c < K / V; ++c) {
+        const int j = c * G * V + lane * V;
+        float x[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (V == 1) x[v] = widen(raw.x[c]);
+            else x[v] = widen(raw.x[c][v]);
+        }
+        if ((c + 1) * G * V > cols) {
+            const int shift = j - (cols - V);           // <= 0: the lane's own entries were read
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                if constexpr (V == 1) h[c] = widen(x);
-                else h[c * V + v] = widen(x[v]);
+                float y = -kInf;
+#pragma unroll
+                for (int w = V - 1; w > v; --w) y = shift == w - v ? x[w] : y;
+                h[c * V + v] = shift <= 0 ? x[v] : y;
             }
         } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[c * V + v] = j + v < cols ? widen(row[j + v]) : -kInf;
+            for (int v = 0; v < V; ++v) h[c * V + v] = x[v];
         }
     }
 }
 
-template <typename E, int K>
+template <typename E, int K, int G = 64>
 __device__ __forceinline__ void store_row(E* row, int lane, int cols, const float (&d)[K])
 {
     constexpr int V = kVec<K>;
     using P = typename Pack<E, V>::type;
 #pragma unroll
     for (int c = 0; c < K / V; ++c) {
-        const int j = c * 64 * V + lane * V;
-        if ((c + 1) * 64 * V <= cols) {
-            P x;
+        const int j = c * G * V + lane * V;
+        P x;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if constexpr (V == 1) x = narrow<E>(d[c]);
-                else x[v] = narrow<E>(d[c * V + v]);
+        for (int v = 0; v < V; ++v) {
+            if constexpr (V == 1) x = narrow<E>(d[c]);
+            else x[v] = narrow<E>(d[c * V + v]);
+        }
+        if (j + V <= cols) *reinterpret_cast<P*>(row + j) = x;
+        if constexpr (V > 1) {
+            if ((c + 1) * G * V > cols && cols % V) {
+#pragma unroll
+                for (int v = 0; v < V - 1; ++v)
+                    if (j + V > cols && j + v < cols) row[j + v] = x[v];
             }
-            *reinterpret_cast<P*>(row + j) = x;
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (j + v < cols) row[j + v] = narrow<E>(d[c * V + v]);
         }
     }
 }
 
 // The column of register i of this lane.
-template <int K>
+template <int K, int G = 64>
 __device__ __forceinline__ int column(int i, int lane)
 {
     constexpr int V = kVec<K>;
-    return (i / V) * 64 * V + lane * V + i % V;
+    return (i / V) * G * V + lane * V + i % V;
 }
 
 // ---- sums over the 64 lanes, four values at a time
@@ -198,43 +227,70 @@ __device__ __forceinline__ float lane_value(float x, int lane)
 // What the exponentials are relative to: an empty row's maximum is -inf, which no entry may be subtracted from.
 __device__ __forceinline__ float base_of(float top) { return top == -kInf ? 0.0f : top; }
 
+__device__ __forceinline__ float sum64(float v)
+{
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// exp(x) 2^60 of a difference x <= 0.  Far below 0 the scale goes into the argument, where float does not flush yet.
+__device__ __forceinline__ float scaled_exp(float x)
+{
+    x *= kLog2e;
+    const bool far = x < -40.0f;
+    return __builtin_amdgcn_exp2f(far ? x + 60.0f : x) * (far ? 1.0f : kScale);
+}
+
 // Maximum and sum over a row's open entries by the whole wave: the steps that k_shared cannot see.
-template <typename E>
+template <typename E, int K>
 __device__ void open_sum(const E* row, const float* pos, float when, int n, int lane, float& top, float& total)
 {
-    float m = -kInf;
-    bool nan = false;
-    for (int j = lane; j < n; j += 64) {
-        const float x = pos[j] > when ? widen(row[j]) : -kInf;
-        nan |= x != x;
-        m = fmaxf(m, x);
+    top = -kInf;
+    total = 0.0f;
+    for (int c = 0; c < n; c += 64 * K) {
+        const int cols = min(64 * K, n - c);
+        Row<E, K> raw;
+        Row<float, K> raw_pos;
+        load_row<E, K>(row + c, lane, cols, raw);
+        load_row<float, K>(pos + c, lane, cols, raw_pos);
+        float h[K], at[K], m = -kInf, s = 0.0f;
+        end_row<E, K>(raw, lane, cols, h);
+        end_row<float, K>(raw_pos, lane, cols, at);
+#pragma unroll
+        for (int x = 0; x < K; ++x) {
+            h[x] = at[x] > when ? h[x] : -kInf;
+            m = fmaxf(m, h[x]);
+        }
+        const float now = fmaxf(top, row_max(m)), from = base_of(now);
+#pragma unroll
+        for (int x = 0; x < K; ++x) s += __builtin_amdgcn_exp2f((h[x] - from) * kLog2e);
+        if (total != 0.0f) total *= __builtin_amdgcn_exp2f((top - from) * kLog2e);
+        total += sum64(s);
+        top = now;
     }
-    top = row_max(m);
-    float s = 0.0f;
-    for (int j = lane; j < n; j += 64)
-        if (pos[j] > when) s += __builtin_amdgcn_exp2f((widen(row[j]) - base_of(top)) * kLog2e);
-    s = wave_sum(s);
-    total = __any(nan) ? __builtin_nanf("") : s;
 }
 
-// lp of one step from its row's statistics.
-template <typename E>
-__device__ __forceinline__ float log_prob(const E* row, int next, float top, float total)
-{
-    return total == 0.0f ? -kInf : (widen(row[next]) - base_of(top)) - logf(total);
-}
-
-// Ends the steps of the lanes with `valid`: (tour k, row r, step t).  Those whose shared sum says nothing are redone
-// one after the other by the whole wave; all lanes have to be here.
-template <typename E, bool SHARED>
+// Ends the steps of the lanes with `valid`: (tour k, row r, step `when`).  `total` is 2^60 times the sum where it is
+// shared.  Steps of which a shared sum says nothing are redone one after the other by the whole wave: all lanes have to
+// be here.
+template <typename E, int K, bool SHARED>
 __device__ void end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, int r, float when, float top,
                           float total, int lane)
 {
     const E* base = static_cast<const E*>(p.logits);
     const E* row = base + map * p.map_stride + (int64_t)r * p.row_stride;
     const int t = (int)when;
-    int next = 0;
-    if (valid) next = p.by_step ? (int)p.tours[k * (p.n + 1) + t + 1] : p.next[k * p.n + r];
+    float chosen = 0.0f;
+    if (valid) chosen = widen(row[p.by_step ? (int)p.tours[k * (p.n + 1) + t + 1] : (int)p.next[k * p.n + r]]);
+    // log(total) and not of total 2^-60 where that would leave the range of float
+    float log_total = logf(!SHARED ? total : total >= 0x1p-60f ? total * (1.0f / kScale) : total);
+    if (SHARED && total < 0x1p-60f) log_total -= 60.0f / kLog2e;
     if constexpr (SHARED) {
         uint64_t redo = __ballot(valid && !(total >= kSmall));
         while (redo) {
@@ -242,14 +298,40 @@ __device__ void end_steps(const LogpParams& p, bool valid, int64_t map, int64_t 
             redo &= redo - 1;
             const int64_t kk = ((int64_t)__builtin_amdgcn_readlane((int)(k >> 32), l) << 32) |
                                (unsigned)__builtin_amdgcn_readlane((int)k, l);
+            const int64_t mm = ((int64_t)__builtin_amdgcn_readlane((int)(map >> 32), l) << 32) |
+                               (unsigned)__builtin_amdgcn_readlane((int)map, l);
             const int rr = __builtin_amdgcn_readlane(r, l);
             float m, s;
-            open_sum(base + (kk / p.per) * p.map_stride + (int64_t)rr * p.row_stride, p.pos + kk * p.n,
-                     lane_value(when, l), p.n, lane, m, s);
-            if (lane == l) { top = m; total = s; }
+            open_sum<E, K>(base + mm * p.map_stride + (int64_t)rr * p.row_stride, p.pos + kk * p.n, lane_value(when, l),
+                           p.n, lane, m, s);
+            if (lane == l) { top = m; total = s; log_total = logf(s); }
         }
     }
-    if (valid) p.logp[k * (p.n - 1) + t] = log_prob(row, next, top, total);
+    if (valid) p.logp[k * (p.n - 1) + t] = total == 0.0f ? -kInf : (chosen - base_of(top)) - log_total;
+}
+
+// The positions of a pass's tours in LDS, a wave a tour.
+template <int K>
+__device__ __forceinline__ void stage(float* tile, const float* pos, int count, int n, int col0, int cols, int wave, int lane)
+{
+    constexpr int V = kVec<K>, per_wave = kTile / kWaves;
+    Row<float, K> raw[per_wave];
+#pragma unroll
+    for (int a = 0; a < per_wave; ++a) {
+        const int q = min(a * kWaves + wave, count - 1);
+        load_row<float, K>(pos + (int64_t)q * n + col0, lane, cols, raw[a]);
+    }
+#pragma unroll
+    for (int a = 0; a < per_wave; ++a) {
+        const int q = a * kWaves + wave;
+        if (q >= count) break;
+        float at[K];
+        end_row<float, K>(raw[a], lane, cols, at);      // behind the end: -inf, which no step comes before
+#pragma unroll
+        for (int c = 0; c < K / V; ++c)
+#pragma unroll
+            for (int v = 0; v < V; ++v) tile[q * 64 * K + c * 64 * V + lane * V + v] = fmaxf(at[c * V + v], -1.0f);
+    }
 }
 
 template <typename E, int K>
@@ -267,31 +349,26 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared(LogpParams p)
     const E* row0 = static_cast<const E*>(p.logits) + map * p.map_stride + col0;
 
     float e[kRows][K], top[kRows];
+    Row<E, K> raw[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) load_row<E, K>(row0 + (int64_t)min(r0 + r, p.n - 1) * p.row_stride, lane, cols, raw[r]);
+    stage<K>(tile, p.pos + map * p.per * (int64_t)p.n, min(kTile, p.per), p.n, col0, cols, wave, lane);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        const int i = r0 + r;
-        if (i < p.n) {
-            load_row<E, K>(row0 + (int64_t)i * p.row_stride, lane, cols, e[r]);
-            const int self = i - col0;                  // the diagonal is never open: it must not set the maximum
-            if (self >= 0 && self < cols) {
+        end_row<E, K>(raw[r], lane, cols, e[r]);
+        const int self = r0 + r - col0;                 // the diagonal is never open: it must not set the maximum
+        if (self >= 0 && self < cols) {
 #pragma unroll
-                for (int x = 0; x < K; ++x)
-                    if (column<K>(x, lane) == self) e[r][x] = -kInf;
-            }
-        } else {
-#pragma unroll
-            for (int x = 0; x < K; ++x) e[r][x] = -kInf;
+            for (int x = 0; x < K; ++x)
+                if (column<K>(x, lane) == self) e[r][x] = -kInf;
         }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
         float m = e[r][0];
 #pragma unroll
         for (int x = 1; x < K; ++x) m = fmaxf(m, e[r][x]);
         top[r] = row_max(m);
         const float from = base_of(top[r]);
 #pragma unroll
-        for (int x = 0; x < K; ++x) e[r][x] = __builtin_amdgcn_exp2f((e[r][x] - from) * kLog2e);
+        for (int x = 0; x < K; ++x) e[r][x] = scaled_exp(e[r][x] - from);
     }
     const float mine = (lane & 2) ? ((lane & 1) ? top[3] : top[2]) : ((lane & 1) ? top[1] : top[0]);
     const int i = r0 + (lane & 3);
@@ -300,10 +377,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared(LogpParams p)
     for (int q0 = 0; q0 < p.per; q0 += kTile) {
         const int count = min(kTile, p.per - q0);
         const float* pos = p.pos + (map * p.per + q0) * (int64_t)p.n;
-        __syncthreads();
-        for (int x = threadIdx.x; x < count * 64 * K; x += 64 * kWaves) {
-            const int q = x / (64 * K), j = x % (64 * K);
-            tile[x] = j < cols ? pos[(int64_t)q * p.n + col0 + j] : -1.0f;
+        if (q0) {
+            __syncthreads();
+            stage<K>(tile, pos, count, p.n, col0, cols, wave, lane);
         }
         // lane = (tour q0 + lane / 4, row lane % 4): the step at which the tour leaves the row's node
         const int q = lane >> 2;
@@ -337,17 +413,17 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared(LogpParams p)
         const int64_t k = map * p.per + q0 + q;
         if (in) (p.parts == 1 ? p.total : p.part_total + (int64_t)part * p.maps * p.per * p.n)[k * p.n + i] = total;
         if (p.parts == 1)
-            end_steps<E, true>(p, in && t >= 0.0f && t < (float)(p.n - 1), map, k, i, t, mine, total, lane);
+            end_steps<E, K, true>(p, in && t >= 0.0f && t < (float)(p.n - 1), map, k, i, t, mine, total, lane);
     }
 }
 
 template <typename E, int K>
 __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
 {
-    extern __shared__ float tile[];                     // [tours of a pass][64 K] positions, then [waves][64 K]
+    extern __shared__ float tile[];                     // [tours of a pass][64 K] positions; in the end [waves][64 K]
     __shared__ float4 when[kWaves][kTile], weight[kWaves][kTile];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    float* hits = tile + p.tile * 64 * K + wave * 64 * K;
+    float* hits = tile + wave * 64 * K;
     const int64_t b = work_block();
     const int part = (int)(b % p.parts);
     const int64_t group = b / p.parts, map = group / p.groups;
@@ -365,11 +441,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
     for (int q0 = 0; q0 < p.per; q0 += kTile) {
         const int count = min(kTile, p.per - q0);
         const float* pos = p.pos + (map * p.per + q0) * (int64_t)p.n;
-        __syncthreads();
-        for (int x = threadIdx.x; x < count * 64 * K; x += 64 * kWaves) {
-            const int q = x / (64 * K), j = x % (64 * K);
-            tile[x] = j < cols ? pos[(int64_t)q * p.n + col0 + j] : -1.0f;
-        }
+        if (q0) __syncthreads();
+        stage<K>(tile, pos, count, p.n, col0, cols, wave, lane);
         const int q = lane >> 2;
         const bool in = q < count && i < p.n;
         const int64_t k = map * p.per + q0 + q;
@@ -399,18 +472,22 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
         }
     }
     const uint64_t redo = __ballot(any_redo);
+    __syncthreads();
+    Row<E, K> raw[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) load_row<E, K>(row0 + (int64_t)min(r0 + r, p.n - 1) * p.row_stride, lane, cols, raw[r]);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const int ii = r0 + r;
         if (ii >= p.n) break;
         const E* row = row0 + (int64_t)ii * p.row_stride;
         float h[K], d[K];
-        load_row<E, K>(row, lane, cols, h);
+        end_row<E, K>(raw[r], lane, cols, h);
         const float from = base_of(p.top[map * p.n + ii]);
         // an entry that no tour had open may hold anything: its weight is 0, and so is its gradient
 #pragma unroll
         for (int x = 0; x < K; ++x)
-            d[x] = sum[r][x] != 0.0f ? -sum[r][x] * __builtin_amdgcn_exp2f((h[x] - from) * kLog2e) : 0.0f;
+            d[x] = sum[r][x] != 0.0f ? -sum[r][x] * scaled_exp(h[x] - from) : 0.0f;
         // + g at the chosen entries.  Tours of one map often choose the same one: they are added one after the other,
         // in their order, by one lane at a time.
 #pragma unroll
@@ -441,7 +518,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
                     const int64_t kk = map * p.per + q0 + l;
                     const float tt = lane_value(t, l), gg = lane_value(g, l);
                     float m, s;
-                    open_sum(row - col0, p.pos + kk * p.n, tt, p.n, lane, m, s);
+                    open_sum<E, K>(row - col0, p.pos + kk * p.n, tt, p.n, lane, m, s);
                     if (s == 0.0f) {                    // nothing was open: no choice, no gradient
                         if (lane == l) to = -1;
                         continue;
@@ -459,7 +536,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
             while (chosen) {
                 const int l = __ffsll((unsigned long long)chosen) - 1;
                 chosen &= chosen - 1;
-                if (lane == l) hits[to] += g;
+                if (lane == l) __hip_atomic_fetch_add(&hits[to], g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -498,15 +575,17 @@ __global__ __launch_bounds__(256) void k_single(LogpParams p)
         z0 = z1; z1 = z2; z2 = z3; z3 = 0.0f;
         if (4 * a >= count) continue;
         float h[4][K], s[4], tt[4];
+        Row<E, K> raw[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = min(4 * a + r, count - 1);
-            load_row<E, K>(row0 + (int64_t)(r0 + i) * p.row_stride, lane, cols, h[r]);
+            load_row<E, K>(row0 + (int64_t)(r0 + i) * p.row_stride, lane, cols, raw[r]);
             tt[r] = lane_value(when, 16 * (i >> 2) + (i & 3));
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             float m = -kInf;
+            end_row<E, K>(raw[r], lane, cols, h[r]);
 #pragma unroll
             for (int x = 0; x < K; ++x) {
                 h[r][x] = pos[x] > tt[r] ? h[r][x] : -kInf;
@@ -530,7 +609,7 @@ __global__ __launch_bounds__(256) void k_single(LogpParams p)
         (p.parts == 1 ? p.total : p.part_total + (int64_t)part * p.maps * p.rows)[at] = total;
     }
     if (p.parts == 1)
-        end_steps<E, false>(p, writes && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), k, k, r0 + mine, when, top,
+        end_steps<E, K, false>(p, writes && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), k, k, r0 + mine, when, top,
                             total, lane);
 }
 
@@ -562,23 +641,31 @@ __global__ __launch_bounds__(256) void k_single_grad(LogpParams p)
             weight = g / total;
         }
     }
-    const E* row0 = static_cast<const E*>(p.logits) + k * p.map_stride + col0;
+    const E* row0 = static_cast<const E*>(p.logits) + k * p.map_stride + r0 * p.row_stride + col0;
     E* out0 = static_cast<E*>(p.grad) + (k * p.rows + r0) * (int64_t)p.n + col0;
-    for (int r = 0; r < count; ++r) {
-        const float tt = lane_value(when, r), ff = lane_value(from, r), ww = lane_value(weight, r), gg = lane_value(g, r);
-        float d[K];
-        if (gg == 0.0f) {                               // whatever the row holds
+    for (int r0 = 0; r0 < count; r0 += 2) {             // two rows in flight
+        Row<E, K> raw[2];
 #pragma unroll
-            for (int x = 0; x < K; ++x) d[x] = 0.0f;
-        } else {
-            load_row<E, K>(row0 + (int64_t)(r0 + r) * p.row_stride, lane, cols, d);
+        for (int a = 0; a < 2; ++a) load_row<E, K>(row0 + (int64_t)min(r0 + a, count - 1) * p.row_stride, lane, cols, raw[a]);
 #pragma unroll
-            for (int x = 0; x < K; ++x) {
-                const float y = -ww * __builtin_amdgcn_exp2f((d[x] - ff) * kLog2e);
-                d[x] = pos[x] > tt ? (pos[x] == tt + 1.0f ? y + gg : y) : 0.0f;
+        for (int a = 0; a < 2; ++a) {
+            const int r = r0 + a;
+            if (r >= count) break;
+            const float tt = lane_value(when, r), ff = lane_value(from, r), ww = lane_value(weight, r), gg = lane_value(g, r);
+            float d[K];
+            end_row<E, K>(raw[a], lane, cols, d);
+            if (gg == 0.0f) {                           // whatever the row holds
+#pragma unroll
+                for (int x = 0; x < K; ++x) d[x] = 0.0f;
+            } else {
+#pragma unroll
+                for (int x = 0; x < K; ++x) {
+                    const float y = -ww * __builtin_amdgcn_exp2f((d[x] - ff) * kLog2e);
+                    d[x] = pos[x] > tt ? (pos[x] == tt + 1.0f ? y + gg : y) : 0.0f;
+                }
             }
+            store_row<E, K>(out0 + (int64_t)r * p.n, lane, cols, d);
         }
-        store_row<E, K>(out0 + (int64_t)r * p.n, lane, cols, d);
     }
 }
 
@@ -597,13 +684,17 @@ __global__ __launch_bounds__(256) void k_join(LogpParams p)
         for (int c = 0; c < p.parts; ++c) top = fmaxf(top, p.part_top[c * p.maps * p.rows + row]);
         for (int c = 0; c < p.parts; ++c) {
             const float m = base_of(p.part_top[c * p.maps * p.rows + row]), s = p.part_total[c * all + w];
-            if (s != 0.0f) total += s * __builtin_amdgcn_exp2f((m - base_of(top)) * kLog2e);
+            const float x = (m - base_of(top)) * kLog2e;
+            if (s == 0.0f) continue;
+            // a shared sum is up to 2^76 and counts down to 2^-80: its factor must not be flushed before it is applied
+            total += SHARED && x < -40.0f ? s * __builtin_amdgcn_exp2f(x + 60.0f) * (1.0f / kScale)
+                                          : s * __builtin_amdgcn_exp2f(x);
         }
         p.total[w] = total;
         if (!SHARED || k % p.per == 0) p.top[row] = top;
     }
     const float when = in ? (p.by_step ? (float)r : p.pos[k * p.n + r]) : 0.0f;
-    end_steps<E, SHARED>(p, in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), SHARED ? k / p.per : k, k, r, when,
+    end_steps<E, kMaxPer, SHARED>(p, in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), SHARED ? k / p.per : k, k, r, when,
                          top, total, lane);
 }
 
@@ -651,7 +742,7 @@ int logp_launch(LogpParams p, bool grad, hipStream_t stream)
     if (grid > 0x7fffffffll) return fail(TSP2OPT_E_UNSUPPORTED, "too many rows");
     int rc = 0;
     if (shared) {
-        const size_t lds = sizeof(float) * 64 * k * (p.tile + (grad ? kWaves : 0));
+        const size_t lds = sizeof(float) * 64 * k * (grad && p.tile < kWaves ? kWaves : p.tile);
         if (grad) T2O_BY_HELD(k, (rc = shared_launch(k_shared_grad<E, K>, p, (unsigned)grid, lds, stream)))
         else T2O_BY_HELD(k, (rc = shared_launch(k_shared<E, K>, p, (unsigned)grid, lds, stream)))
     } else {
@@ -756,7 +847,7 @@ extern "C" int tsp2opt_tour_logprobs(const void* logits, const int64_t* tours, f
     if (lds > 48 * 1024)
         HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(k_positions),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    const unsigned threads = n <= 64 ? 64 : n <= 128 ? 128 : 256;
+    const unsigned threads = n <= 64 ? 64 : n <= 128 ? 128 : n <= 1024 ? 256 : 1024;
     hipLaunchKernelGGL(k_positions, dim3((unsigned)num_tours), dim3(threads), lds, stream, tours, p.pos, p.next, logp_out,
                        n);
     int result = 0;
