@@ -7,8 +7,9 @@
 // autoregressive decoder wrote.  Gradient, with g(t) the gradient of lp(t):
 //     dh[r, j] = sum over the tours that share the row of  g(t) ([j = tour[t+1]] - [pos(j) > t] softmax_j).
 //
-// Every wave keeps (part of) its rows in registers: K entries of a row a lane, 64 K columns, loaded once.  Rows longer
-// than 1024 entries are split into parts whose maxima and sums k_join puts together.
+// Rows are kept in registers, K entries a lane, loaded once.  A row of up to 256 entries takes G = 16 lanes (four rows
+// side by side in a wave: sums over 16 lanes need no cross-row steps), longer ones G = 64; rows of more than 1024 are
+// split into parts whose maxima and sums k_join puts together.
 //
 // Several tours a map (k_shared): e_j = exp(h_j - row maximum) does not depend on the tour, only which e_j are added
 // does, and positions are whole numbers, so a masked addition is
@@ -20,14 +21,18 @@
 // One tour a row (k_single): the maximum is the open entries' own, nothing is ever lost.
 #include "learn_common.hpp"
 
+#include <type_traits>
+
 namespace t2o {
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kSmall = 0x1p-80f, kScale = 0x1p60f;
-constexpr int kWaves = 8, kRows = 4, kTile = 16;    // k_shared: waves a workgroup, rows a wave, tours a pass
+constexpr float kDead = -1.0f;                      // k_shared's total of a step with no open entry
+constexpr int kRows = 4, kTile = 16;                // k_shared: rows of a group of lanes, tours a pass
 constexpr int kSingleRows = 16;                     // k_single: rows a wave
 constexpr int kMaxPer = 16;                         // entries of a row a lane holds at most
+constexpr int kShortRow = 256;                      // longest row of a group of 16 lanes
 
 struct LogpParams {
     const void* logits;
@@ -36,13 +41,13 @@ struct LogpParams {
     float* pos;             // (T, n); -1 everywhere: the tour is no permutation
     uint16_t* next;         // (T, n): the node after a node
     float* top;             // (M, rows) shared, (T, rows) single: what the exponentials are relative to
-    float* total;           // (T, rows): sum of exp(h - top) over the open entries
+    float* total;           // (T, rows): sum of exp(h - top) over the open entries (shared: times 2^60)
     float* part_top;        // [parts](M or T, rows)
     float* part_total;      // [parts](T, rows)
     const float* g;         // (T, n - 1)
     void* grad;             // (M, rows, n)
     int64_t maps, map_stride, row_stride, groups;
-    int32_t n, rows, per, by_step, parts, tile;
+    int32_t n, rows, per, by_step, parts;
 };
 
 // Consecutive workgroups go to the eight dies in turn; this gives each die a contiguous range of the work instead, so
@@ -80,8 +85,8 @@ __global__ __launch_bounds__(1024) void k_positions(const int64_t* tours, float*
         for (int s = threadIdx.x; s < n - 1; s += blockDim.x) logp[k * (n - 1) + s] = __builtin_nanf("");
 }
 
-// ---- rows in registers: lane l holds entries c * 64 V + l V + v, V adjacent ones a load.  Rows of odd length start
-// anywhere, so the loads are aligned to the element only, which the memory pipe takes at full width.
+// ---- rows in registers: lane l of a group of G holds entries c G V + l V + v, V adjacent ones a load.  Rows of odd
+// length start anywhere, so the loads are aligned to the element only, which the memory pipe takes at full width.
 template <int K>
 constexpr int kVec = K % 4 == 0 ? 4 : K % 2 == 0 ? 2 : 1;
 
@@ -98,37 +103,38 @@ struct Pack<E, 1> {
 // short last part there is the previous one) and end_row puts its entries in place.
 template <typename E, int K>
 struct Row {
-    static constexpr int V = kVec<K>;
-    typename Pack<E, V>::type x[K / V];
+    typename Pack<E, kVec<K>>::type x[K / kVec<K>];
 };
 
-template <typename E, int K, int G = 64>
-__device__ __forceinline__ void load_row(const E* row, int lane, int cols, Row<E, K>& raw)
+template <typename E, int K, int G>
+__device__ __forceinline__ void load_row(const E* row, int l, int cols, Row<E, K>& raw)
 {
     constexpr int V = kVec<K>;
     using P = typename Pack<E, V>::type;
 #pragma unroll
-    for (int c = 0; c < K / V; ++c) {
-        const int j = c * G * V + lane * V;
-        raw.x[c] = *reinterpret_cast<const P*>(row + min(j, cols - V));
-    }
+    for (int c = 0; c < K / V; ++c) raw.x[c] = *reinterpret_cast<const P*>(row + min(c * G * V + l * V, cols - V));
 }
 
-template <typename E, int K, int G = 64>
-__device__ __forceinline__ void end_row(const Row<E, K>& raw, int lane, int cols, float (&h)[K])
+template <typename E, int K, int G>
+__device__ __forceinline__ void end_row(const Row<E, K>& raw, int l, int cols, float (&h)[K])
 {
     constexpr int V = kVec<K>;
 #pragma unroll
     for (int c = 0; c < K / V; ++c) {
-        const int j = c * G * V + lane * V;
-        float x[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if constexpr (V == 1) x[v] = widen(raw.x[c]);
-            else x[v] = widen(raw.x[c][v]);
+            if constexpr (V == 1) h[c] = widen(raw.x[c]);
+            else h[c * V + v] = widen(raw.x[c][v]);
         }
-        if ((c + 1) * G * V > cols) {
-            const int shift = j - (cols - V);           // <= 0: the lane's own entries were read
+        if ((c + 1) * G * V <= cols) continue;
+        const int shift = c * G * V + l * V - (cols - V);       // <= 0: the lane's own entries were read
+        if (cols % V == 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[c * V + v] = shift <= 0 ? h[c * V + v] : -kInf;
+        } else {
+            float x[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = h[c * V + v];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float y = -kInf;
@@ -136,21 +142,18 @@ __device__ __forceinline__ void end_row(const Row<E, K>& raw, int lane, int cols
                 for (int w = V - 1; w > v; --w) y = shift == w - v ? x[w] : y;
                 h[c * V + v] = shift <= 0 ? x[v] : y;
             }
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[c * V + v] = x[v];
         }
     }
 }
 
-template <typename E, int K, int G = 64>
-__device__ __forceinline__ void store_row(E* row, int lane, int cols, const float (&d)[K])
+template <typename E, int K, int G>
+__device__ __forceinline__ void store_row(E* row, int l, int cols, const float (&d)[K])
 {
     constexpr int V = kVec<K>;
     using P = typename Pack<E, V>::type;
 #pragma unroll
     for (int c = 0; c < K / V; ++c) {
-        const int j = c * G * V + lane * V;
+        const int j = c * G * V + l * V;
         P x;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -168,15 +171,15 @@ __device__ __forceinline__ void store_row(E* row, int lane, int cols, const floa
     }
 }
 
-// The column of register i of this lane.
-template <int K, int G = 64>
-__device__ __forceinline__ int column(int i, int lane)
+// The column of register i of lane l.
+template <int K, int G>
+__device__ __forceinline__ int column(int i, int l)
 {
     constexpr int V = kVec<K>;
-    return (i / V) * G * V + lane * V + i % V;
+    return (i / V) * G * V + l * V + i % V;
 }
 
-// ---- sums over the 64 lanes, four values at a time
+// ---- sums and maxima over the G lanes of a group
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x)
 {
@@ -184,39 +187,78 @@ __device__ __forceinline__ float dpp(float x)
     return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
 }
 
-// a[0..3] -> value (lane & 3) summed over the 16 lanes of this lane's row, in every lane of that row
-__device__ __forceinline__ float quad_sum(const float (&a)[4], bool odd, bool high)
+// fmaxf quiets its operands first; these are one instruction.  A NaN operand is left out, as fmaxf leaves it out.
+__device__ __forceinline__ float vmax(float a, float b)
 {
-    const float u = (odd ? a[1] : a[0]) + dpp<0xB1>(odd ? a[0] : a[1]);         // quad_perm [1,0,3,2]
-    const float v = (odd ? a[3] : a[2]) + dpp<0xB1>(odd ? a[2] : a[3]);
-    float w = (high ? v : u) + dpp<0x4E>(high ? u : v);                         // quad_perm [2,3,0,1]
-    w += dpp<0x124>(w);                                                         // row_ror:4
-    return w + dpp<0x128>(w);                                                   // row_ror:8
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
+__device__ __forceinline__ float vmax3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+template <int K>
+__device__ __forceinline__ float max_of(const float (&h)[K])
+{
+    if constexpr (K == 1) return h[0];
+    float m = vmax(h[0], h[1]);
+#pragma unroll
+    for (int x = 2; x + 1 < K; x += 2) m = vmax3(m, h[x], h[x + 1]);
+    return m;                                           // K is 1 or even
+}
+
+template <typename F>
+__device__ __forceinline__ float swap16(float a, float b, F f)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <typename F>
+__device__ __forceinline__ float swap32(float a, float b, F f)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+struct Add {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+    __device__ __forceinline__ float operator()(float a, float b) const { return vmax(a, b); }
+};
+
+template <int G, typename F>
+__device__ __forceinline__ float all(float v, F f)
+{
+    v = f(v, dpp<0xB1>(v));                             // quad_perm [1,0,3,2]
+    v = f(v, dpp<0x4E>(v));                             // quad_perm [2,3,0,1]
+    v = f(v, dpp<0x141>(v));                            // row_half_mirror
+    v = f(v, dpp<0x140>(v));                            // row_mirror
+    if constexpr (G == 64) v = swap32(swap16(v, v, f), swap16(v, v, f), f);
+    return v;
+}
+
+// a[0..3] -> value (lane & 3) over the 16 lanes of this lane's row, in every lane of that row
+template <typename F>
+__device__ __forceinline__ float quads(const float (&a)[4], bool odd, bool high, F f)
+{
+    const float u = f(odd ? a[1] : a[0], dpp<0xB1>(odd ? a[0] : a[1]));
+    const float v = f(odd ? a[3] : a[2], dpp<0xB1>(odd ? a[2] : a[3]));
+    float w = f(high ? v : u, dpp<0x4E>(high ? u : v));
+    w = f(w, dpp<0x124>(w));                            // row_ror:4
+    return f(w, dpp<0x128>(w));                         // row_ror:8
 }
 
 // z0..z3 -> z(lane >> 4) summed over the four rows of 16 lanes
 __device__ __forceinline__ float rows_sum(float z0, float z1, float z2, float z3)
 {
-    auto swap16 = [](float a, float b) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    };
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(swap16(z0, z1)), __float_as_uint(swap16(z2, z3)),
-                                                    false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-__device__ __forceinline__ float row_max(float m)
-{
-    m = fmaxf(m, dpp<0xB1>(m));
-    m = fmaxf(m, dpp<0x4E>(m));
-    m = fmaxf(m, dpp<0x141>(m));                                                // row_half_mirror
-    m = fmaxf(m, dpp<0x140>(m));                                                // row_mirror
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-    m = fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(m)));
+    return swap32(swap16(z0, z1, Add()), swap16(z2, z3, Add()), Add());
 }
 
 __device__ __forceinline__ float lane_value(float x, int lane)
@@ -227,210 +269,318 @@ __device__ __forceinline__ float lane_value(float x, int lane)
 // What the exponentials are relative to: an empty row's maximum is -inf, which no entry may be subtracted from.
 __device__ __forceinline__ float base_of(float top) { return top == -kInf ? 0.0f : top; }
 
-__device__ __forceinline__ float sum64(float v)
-{
-    v += dpp<0xB1>(v);
-    v += dpp<0x4E>(v);
-    v += dpp<0x141>(v);
-    v += dpp<0x140>(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// exp(x) 2^60 of a difference x <= 0.  Far below 0 the scale goes into the argument, where float does not flush yet.
+// exp(x) 2^60 of a difference x <= 0, down to where exp(x) 2^60 itself is flushed: as the square of exp(x / 2) 2^30.
 __device__ __forceinline__ float scaled_exp(float x)
 {
-    x *= kLog2e;
-    const bool far = x < -40.0f;
-    return __builtin_amdgcn_exp2f(far ? x + 60.0f : x) * (far ? 1.0f : kScale);
+    const float y = __builtin_amdgcn_exp2f(x * (0.5f * kLog2e)) * 0x1p30f;
+    return y * y;
 }
 
-// Maximum and sum over a row's open entries by the whole wave: the steps that k_shared cannot see.
-template <typename E, int K>
-__device__ void open_sum(const E* row, const float* pos, float when, int n, int lane, float& top, float& total)
+__device__ __forceinline__ float plain_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// Maximum and sum over a row's open entries by a group of lanes: the steps that k_shared cannot see.
+template <typename E, int K, int G>
+__device__ void open_sum(const E* row, const float* pos, float when, int n, int l, float& top, float& total)
 {
     top = -kInf;
     total = 0.0f;
-    for (int c = 0; c < n; c += 64 * K) {
-        const int cols = min(64 * K, n - c);
+    for (int c = 0; c < n; c += G * K) {
+        const int cols = min(G * K, n - c);
         Row<E, K> raw;
         Row<float, K> raw_pos;
-        load_row<E, K>(row + c, lane, cols, raw);
-        load_row<float, K>(pos + c, lane, cols, raw_pos);
-        float h[K], at[K], m = -kInf, s = 0.0f;
-        end_row<E, K>(raw, lane, cols, h);
-        end_row<float, K>(raw_pos, lane, cols, at);
+        load_row<E, K, G>(row + c, l, cols, raw);
+        load_row<float, K, G>(pos + c, l, cols, raw_pos);
+        float h[K], at[K], s = 0.0f;
+        end_row<E, K, G>(raw, l, cols, h);
+        end_row<float, K, G>(raw_pos, l, cols, at);
 #pragma unroll
-        for (int x = 0; x < K; ++x) {
-            h[x] = at[x] > when ? h[x] : -kInf;
-            m = fmaxf(m, h[x]);
-        }
-        const float now = fmaxf(top, row_max(m)), from = base_of(now);
+        for (int x = 0; x < K; ++x) h[x] = at[x] > when ? h[x] : -kInf;
+        const float now = vmax(top, all<G>(max_of(h), Max())), from = base_of(now);
 #pragma unroll
-        for (int x = 0; x < K; ++x) s += __builtin_amdgcn_exp2f((h[x] - from) * kLog2e);
-        if (total != 0.0f) total *= __builtin_amdgcn_exp2f((top - from) * kLog2e);
-        total += sum64(s);
+        for (int x = 0; x < K; ++x) s += plain_exp(h[x] - from);
+        if (total != 0.0f) total *= plain_exp(top - from);
+        total += all<G>(s, Add());
         top = now;
     }
 }
 
-// Ends the steps of the lanes with `valid`: (tour k, row r, step `when`).  `total` is 2^60 times the sum where it is
-// shared.  Steps of which a shared sum says nothing are redone one after the other by the whole wave: all lanes have to
-// be here.
-template <typename E, int K, bool SHARED>
-__device__ void end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, int r, float when, float top,
-                          float total, int lane)
+// The group's lanes with `todo`, one after the other: the lane whose turn it is, or -1 when the group is through.
+template <int G>
+struct Turns {
+    uint64_t mask;
+    int first;
+    __device__ Turns(bool todo, int lane) : mask(__ballot(todo)), first(lane & ~(G - 1))
+    {
+        if constexpr (G < 64) mask = (mask >> first) & ((1ull << G) - 1);
+    }
+    __device__ bool more() const { return __any(mask != 0); }
+    __device__ int take()
+    {
+        const int at = __ffsll((unsigned long long)mask) - 1;
+        mask &= mask - 1;
+        return at < 0 ? -1 : first + at;
+    }
+};
+
+__device__ __forceinline__ int64_t shfl64(int64_t x, int src)
+{
+    return ((int64_t)__shfl((int)(x >> 32), src) << 32) | (unsigned)__shfl((int)x, src);
+}
+
+// Ends the steps of the lanes with `valid`: (tour k, row r, step `when`).  A shared total is 2^60 times the sum; steps of
+// which it says nothing are redone one after the other by their group of lanes: all lanes have to be here.  Returns what
+// the gradient needs to know of the step.
+template <typename E, int K, int G, bool SHARED>
+__device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, int r, float when,
+                                           float top, float total, int lane)
 {
     const E* base = static_cast<const E*>(p.logits);
     const E* row = base + map * p.map_stride + (int64_t)r * p.row_stride;
     const int t = (int)when;
-    float chosen = 0.0f;
+    float chosen = 0.0f, keep = total;
     if (valid) chosen = widen(row[p.by_step ? (int)p.tours[k * (p.n + 1) + t + 1] : (int)p.next[k * p.n + r]]);
     // log(total) and not of total 2^-60 where that would leave the range of float
     float log_total = logf(!SHARED ? total : total >= 0x1p-60f ? total * (1.0f / kScale) : total);
     if (SHARED && total < 0x1p-60f) log_total -= 60.0f / kLog2e;
     if constexpr (SHARED) {
-        uint64_t redo = __ballot(valid && !(total >= kSmall));
-        while (redo) {
-            const int l = __ffsll((unsigned long long)redo) - 1;
-            redo &= redo - 1;
-            const int64_t kk = ((int64_t)__builtin_amdgcn_readlane((int)(k >> 32), l) << 32) |
-                               (unsigned)__builtin_amdgcn_readlane((int)k, l);
-            const int64_t mm = ((int64_t)__builtin_amdgcn_readlane((int)(map >> 32), l) << 32) |
-                               (unsigned)__builtin_amdgcn_readlane((int)map, l);
-            const int rr = __builtin_amdgcn_readlane(r, l);
-            float m, s;
-            open_sum<E, K>(base + mm * p.map_stride + (int64_t)rr * p.row_stride, p.pos + kk * p.n, lane_value(when, l),
-                           p.n, lane, m, s);
-            if (lane == l) { top = m; total = s; log_total = logf(s); }
+        for (Turns<G> turns(valid && !(total >= kSmall), lane); turns.more();) {
+            const int turn = turns.take(), src = max(turn, 0);
+            const int64_t kk = shfl64(k, src), mm = shfl64(map, src);
+            const int rr = __shfl(r, src);
+            const float ww = __shfl(when, src);
+            float m = 0.0f, s = 0.0f;
+            if (turn >= 0)
+                open_sum<E, K, G>(base + mm * p.map_stride + (int64_t)rr * p.row_stride, p.pos + kk * p.n, ww, p.n,
+                                  lane & (G - 1), m, s);
+            if (lane == turn) {
+                top = m;
+                total = s;
+                log_total = logf(s);
+                if (s == 0.0f) keep = kDead;
+            }
         }
     }
     if (valid) p.logp[k * (p.n - 1) + t] = total == 0.0f ? -kInf : (chosen - base_of(top)) - log_total;
+    return keep;
 }
 
-// The positions of a pass's tours in LDS, a wave a tour.
-template <int K>
+// ---- several tours a map
+template <int G>
+constexpr int kWaves = G == 64 ? 8 : 4;
+template <int G>
+constexpr int kWaveRows = kRows * 64 / G;               // rows of a wave
+
+// The positions of a pass's tours in LDS, a group of 64 lanes a tour; behind the end of a row: -inf, which is never open.
+template <int K, int G>
 __device__ __forceinline__ void stage(float* tile, const float* pos, int count, int n, int col0, int cols, int wave, int lane)
 {
-    constexpr int V = kVec<K>, per_wave = kTile / kWaves;
-    Row<float, K> raw[per_wave];
+    constexpr int per_wave = kTile / kWaves<G>, C = G * K;
+    if constexpr (G == 64) {
+        constexpr int V = kVec<K>;
+        Row<float, K> raw[per_wave];
 #pragma unroll
-    for (int a = 0; a < per_wave; ++a) {
-        const int q = min(a * kWaves + wave, count - 1);
-        load_row<float, K>(pos + (int64_t)q * n + col0, lane, cols, raw[a]);
-    }
+        for (int a = 0; a < per_wave; ++a) {
+            const int q = min(a * kWaves<G> + wave, count - 1);
+            load_row<float, K, 64>(pos + (int64_t)q * n + col0, lane, cols, raw[a]);
+        }
 #pragma unroll
-    for (int a = 0; a < per_wave; ++a) {
-        const int q = a * kWaves + wave;
-        if (q >= count) break;
-        float at[K];
-        end_row<float, K>(raw[a], lane, cols, at);      // behind the end: -inf, which no step comes before
+        for (int a = 0; a < per_wave; ++a) {
+            const int q = a * kWaves<G> + wave;
+            if (q >= count) break;
+            float at[K];
+            end_row<float, K, 64>(raw[a], lane, cols, at);
 #pragma unroll
-        for (int c = 0; c < K / V; ++c)
+            for (int c = 0; c < K / V; ++c)
 #pragma unroll
-            for (int v = 0; v < V; ++v) tile[q * 64 * K + c * 64 * V + lane * V + v] = fmaxf(at[c * V + v], -1.0f);
+                for (int v = 0; v < V; ++v) tile[q * C + c * 64 * V + lane * V + v] = at[c * V + v];
+        }
+    } else {
+        constexpr int steps = (C + 63) / 64;
+        float x[per_wave][steps];
+#pragma unroll
+        for (int a = 0; a < per_wave; ++a)
+#pragma unroll
+            for (int c = 0; c < steps; ++c)
+                x[a][c] = pos[(int64_t)min(a * kWaves<G> + wave, count - 1) * n + min(c * 64 + lane, cols - 1)];
+#pragma unroll
+        for (int a = 0; a < per_wave; ++a)
+#pragma unroll
+            for (int c = 0; c < steps; ++c) {
+                const int q = a * kWaves<G> + wave, j = c * 64 + lane;
+                if (q < count && j < C) tile[q * C + j] = j < cols ? x[a][c] : -kInf;
+            }
     }
 }
 
-template <typename E, int K>
-__global__ __launch_bounds__(64 * kWaves) void k_shared(LogpParams p)
+// Where a wave's work lies.
+template <int K, int G>
+struct SharedWork {
+    int lane, wave, l, group, part, r0, mine, col0, cols;       // mine: first row of this lane's group of lanes
+    int64_t map;
+    __device__ explicit SharedWork(const LogpParams& p)
+    {
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        l = lane & (G - 1);
+        group = lane / G;
+        const int64_t b = work_block(), block = b / p.parts;
+        part = (int)(b % p.parts);
+        map = block / p.groups;
+        r0 = (int)(block % p.groups) * (kWaves<G> * kWaveRows<G>) + wave * kWaveRows<G>;
+        mine = r0 + group * kRows;
+        col0 = part * G * K;
+        cols = min(G * K, p.n - col0);
+    }
+};
+
+// Bound by its vector instructions: 2 K kRows for the masked additions of a tour, 11 to sum them over 16 lanes (and 2/16
+// of two swaps and an add across), an exponential and 10 more an entry of a row.
+template <typename E, int K, int G>
+__global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 {
-    extern __shared__ float tile[];                     // [tours of a pass][64 K] positions
-    __shared__ float4 when[kWaves][kTile];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t b = work_block();
-    const int part = (int)(b % p.parts);
-    const int64_t group = b / p.parts, map = group / p.groups;
-    const int r0 = (int)(group % p.groups) * (kWaves * kRows) + wave * kRows;
-    const int col0 = part * 64 * K, cols = min(64 * K, p.n - col0);
+    extern __shared__ float tile[];                     // [tours of a pass][G K] positions
+    __shared__ float4 when[kWaves<G>][kTile][64 / G];   // the steps at which the tours leave a wave's rows
+    const SharedWork<K, G> w(p);
+    const int lane = w.lane, l = w.l;
     const bool odd = lane & 1, high = lane & 2;
-    const E* row0 = static_cast<const E*>(p.logits) + map * p.map_stride + col0;
+    const E* row0 = static_cast<const E*>(p.logits) + w.map * p.map_stride + w.col0;
 
     float e[kRows][K], top[kRows];
     Row<E, K> raw[kRows];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) load_row<E, K>(row0 + (int64_t)min(r0 + r, p.n - 1) * p.row_stride, lane, cols, raw[r]);
-    stage<K>(tile, p.pos + map * p.per * (int64_t)p.n, min(kTile, p.per), p.n, col0, cols, wave, lane);
+    for (int r = 0; r < kRows; ++r)
+        load_row<E, K, G>(row0 + (int64_t)min(w.mine + r, p.n - 1) * p.row_stride, l, w.cols, raw[r]);
+    stage<K, G>(tile, p.pos + w.map * p.per * (int64_t)p.n, min(kTile, p.per), p.n, w.col0, w.cols, w.wave, lane);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        end_row<E, K>(raw[r], lane, cols, e[r]);
-        const int self = r0 + r - col0;                 // the diagonal is never open: it must not set the maximum
-        if (self >= 0 && self < cols) {
+        end_row<E, K, G>(raw[r], l, w.cols, e[r]);
+        // the diagonal is never open: it must not set the maximum
+        const int self = w.mine + r - w.col0;
 #pragma unroll
-            for (int x = 0; x < K; ++x)
-                if (column<K>(x, lane) == self) e[r][x] = -kInf;
+        for (int c = 0; c < K; c += kVec<K>) {
+            const int first = column<K, G>(c, 0);
+            if (w.r0 + kWaveRows<G> <= w.col0 + first || w.r0 >= w.col0 + first + G * kVec<K>) continue;
+#pragma unroll
+            for (int v = 0; v < kVec<K>; ++v) e[r][c + v] = column<K, G>(c + v, l) == self ? -kInf : e[r][c + v];
         }
-        float m = e[r][0];
+        top[r] = max_of(e[r]);
+    }
+    float mine = quads(top, odd, high, Max());          // of row lane & 3 of the group
+    if constexpr (G == 64) mine = swap32(swap16(mine, mine, Max()), swap16(mine, mine, Max()), Max());
+    top[0] = dpp<0x00>(mine);                           // quad_perm [r,r,r,r]
+    top[1] = dpp<0x55>(mine);
+    top[2] = dpp<0xAA>(mine);
+    top[3] = dpp<0xFF>(mine);
 #pragma unroll
-        for (int x = 1; x < K; ++x) m = fmaxf(m, e[r][x]);
-        top[r] = row_max(m);
+    for (int r = 0; r < kRows; ++r) {
         const float from = base_of(top[r]);
 #pragma unroll
         for (int x = 0; x < K; ++x) e[r][x] = scaled_exp(e[r][x] - from);
     }
-    const float mine = (lane & 2) ? ((lane & 1) ? top[3] : top[2]) : ((lane & 1) ? top[1] : top[0]);
-    const int i = r0 + (lane & 3);
-    if (lane < kRows && i < p.n) (p.parts == 1 ? p.top : p.part_top + (int64_t)part * p.maps * p.n)[map * p.n + i] = mine;
+    const int i = w.mine + (lane & 3);
+    if (l < kRows && i < p.n)
+        (p.parts == 1 ? p.top : p.part_top + (int64_t)w.part * p.maps * p.n)[w.map * p.n + i] = mine;
+
+    float* const when_of = reinterpret_cast<float*>(when[w.wave]);      // [tour][row of the wave]
+    // lane (tour, row i): its step, and its sum where this is the only part
+    auto finish = [&](int q0, int q, int count, float total) {
+        const float t = when_of[q * kWaveRows<G> + w.group * kRows + (lane & 3)];
+        const bool in = q < count && i < p.n;
+        const int64_t k = w.map * p.per + q0 + q;
+        if (p.parts == 1)
+            total = end_steps<E, K, G, true>(p, in && t >= 0.0f && t < (float)(p.n - 1), w.map, k, i, t, mine, total, lane);
+        if (in) (p.parts == 1 ? p.total : p.part_total + (int64_t)w.part * p.maps * p.per * p.n)[k * p.n + i] = total;
+    };
 
     for (int q0 = 0; q0 < p.per; q0 += kTile) {
         const int count = min(kTile, p.per - q0);
-        const float* pos = p.pos + (map * p.per + q0) * (int64_t)p.n;
+        const float* pos = p.pos + (w.map * p.per + q0) * (int64_t)p.n;
         if (q0) {
             __syncthreads();
-            stage<K>(tile, pos, count, p.n, col0, cols, wave, lane);
+            stage<K, G>(tile, pos, count, p.n, w.col0, w.cols, w.wave, lane);
         }
-        // lane = (tour q0 + lane / 4, row lane % 4): the step at which the tour leaves the row's node
-        const int q = lane >> 2;
-        const bool in = q < count && i < p.n;
-        const float t = in ? pos[(int64_t)q * p.n + i] : 65536.0f;
-        reinterpret_cast<float*>(when[wave])[lane] = t;
+#pragma unroll
+        for (int x = lane; x < kTile * kWaveRows<G>; x += 64) {
+            const int q = x / kWaveRows<G>, r = w.r0 + x % kWaveRows<G>;
+            when_of[x] = q < count && r < p.n ? pos[(int64_t)q * p.n + r] : 65536.0f;
+        }
         __syncthreads();
         float z0 = 0.0f, z1 = 0.0f, z2 = 0.0f, z3 = 0.0f;
         for (int a = 0; a < kTile / 4; ++a) {
             z0 = z1; z1 = z2; z2 = z3; z3 = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int qq = 4 * a + c;
-                if (qq >= count) continue;
-                const float4 tt = when[wave][qq];
-                const float* at = tile + qq * 64 * K;
+                const int q = 4 * a + c;
+                if (q >= count) continue;
+                const float4 tt = when[w.wave][q][w.group];
+                const float* at = tile + q * G * K;
                 float s[kRows] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int x = 0; x < K; ++x) {
-                    const float y = at[column<K>(x, lane)];
+                    const float y = at[column<K, G>(x, l)];
                     s[0] = fmaf(__builtin_amdgcn_fmed3f(y - tt.x, 0.0f, 1.0f), e[0][x], s[0]);
                     s[1] = fmaf(__builtin_amdgcn_fmed3f(y - tt.y, 0.0f, 1.0f), e[1][x], s[1]);
                     s[2] = fmaf(__builtin_amdgcn_fmed3f(y - tt.z, 0.0f, 1.0f), e[2][x], s[2]);
                     s[3] = fmaf(__builtin_amdgcn_fmed3f(y - tt.w, 0.0f, 1.0f), e[3][x], s[3]);
                 }
-                const float w = quad_sum(s, odd, high);
-                z3 = ((lane >> 2) & 3) == c ? w : z3;
+                const float sum = quads(s, odd, high, Add());
+                z3 = ((lane >> 2) & 3) == c ? sum : z3;
+            }
+            if constexpr (G == 16) {
+                if (4 * a < count) finish(q0, 4 * a + ((lane >> 2) & 3), count, z3);
             }
         }
-        const float total = rows_sum(z0, z1, z2, z3);
-        const int64_t k = map * p.per + q0 + q;
-        if (in) (p.parts == 1 ? p.total : p.part_total + (int64_t)part * p.maps * p.per * p.n)[k * p.n + i] = total;
-        if (p.parts == 1)
-            end_steps<E, K, true>(p, in && t >= 0.0f && t < (float)(p.n - 1), map, k, i, t, mine, total, lane);
+        if constexpr (G == 64) finish(q0, lane >> 2, count, rows_sum(z0, z1, z2, z3));
     }
 }
 
-template <typename E, int K>
-__global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
+// Equal targets among 16 lanes: their values are added up, nearest first, in the last lane of them; the others get -1.
+__device__ __forceinline__ void join_equal(int& to, float& g)
 {
-    extern __shared__ float tile[];                     // [tours of a pass][64 K] positions; in the end [waves][64 K]
-    __shared__ float4 when[kWaves][kTile], weight[kWaves][kTile];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    float* hits = tile + wave * 64 * K;
-    const int64_t b = work_block();
-    const int part = (int)(b % p.parts);
-    const int64_t group = b / p.parts, map = group / p.groups;
-    const int r0 = (int)(group % p.groups) * (kWaves * kRows) + wave * kRows;
-    const int col0 = part * 64 * K, cols = min(64 * K, p.n - col0);
-    const E* row0 = static_cast<const E*>(p.logits) + map * p.map_stride + col0;
-    const int i = r0 + (lane & 3);
+    bool later = false;
+    float sum = g;
+    auto step = [&](auto shift) {
+        constexpr int D = decltype(shift)::value;
+        const int before = __builtin_amdgcn_update_dpp(-2, to, 0x110 + D, 0xf, 0xf, false);         // row_shr
+        const int behind = __builtin_amdgcn_update_dpp(-2, to, 0x100 + D, 0xf, 0xf, false);         // row_shl
+        const float x = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(g), 0x110 + D, 0xf, 0xf, false));
+        sum += before == to ? x : 0.0f;
+        later |= behind == to;
+    };
+    step(std::integral_constant<int, 1>()); step(std::integral_constant<int, 2>()); step(std::integral_constant<int, 3>());
+    step(std::integral_constant<int, 4>()); step(std::integral_constant<int, 5>()); step(std::integral_constant<int, 6>());
+    step(std::integral_constant<int, 7>()); step(std::integral_constant<int, 8>()); step(std::integral_constant<int, 9>());
+    step(std::integral_constant<int, 10>()); step(std::integral_constant<int, 11>()); step(std::integral_constant<int, 12>());
+    step(std::integral_constant<int, 13>()); step(std::integral_constant<int, 14>()); step(std::integral_constant<int, 15>());
+    g = sum;
+    if (later) to = -1;
+}
+
+template <typename E, int K, int G>
+__global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
+{
+    extern __shared__ float tile[];                     // [tours of a pass][G K] positions; in the end [waves][64 K]
+    __shared__ float4 when[kWaves<G>][kTile][64 / G], weight[kWaves<G>][kTile][64 / G];
+    const SharedWork<K, G> w(p);
+    const int lane = w.lane, l = w.l;
+    const E* row0 = static_cast<const E*>(p.logits) + w.map * p.map_stride + w.col0;
+    // what the gradient of tour q's step that leaves row i takes; g = 0: nothing
+    struct Step {
+        float t, g, total;
+        int to;
+    };
+    auto step_of = [&](int q, int i, bool want_to) {
+        Step s{65536.0f, 0.0f, 0.0f, -1};
+        if (q >= p.per || i >= p.n) return s;
+        const int64_t k = w.map * p.per + q;
+        s.t = p.pos[k * p.n + i];
+        if (!(s.t >= 0.0f && s.t < (float)(p.n - 1))) return s;
+        s.total = p.total[k * p.n + i];
+        if (s.total != kDead) s.g = p.g[k * (p.n - 1) + (int)s.t];
+        if (want_to && s.g != 0.0f) s.to = (int)p.next[k * p.n + i] - w.col0;
+        return s;
+    };
+    auto unseen = [](const Step& s) { return s.g != 0.0f && (!(s.total >= kSmall) || !(fabsf(s.g / s.total) < kInf)); };
 
     float sum[kRows][K];
 #pragma unroll
@@ -440,30 +590,23 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
     bool any_redo = false;
     for (int q0 = 0; q0 < p.per; q0 += kTile) {
         const int count = min(kTile, p.per - q0);
-        const float* pos = p.pos + (map * p.per + q0) * (int64_t)p.n;
         if (q0) __syncthreads();
-        stage<K>(tile, pos, count, p.n, col0, cols, wave, lane);
-        const int q = lane >> 2;
-        const bool in = q < count && i < p.n;
-        const int64_t k = map * p.per + q0 + q;
-        const float t = in ? pos[(int64_t)q * p.n + i] : 65536.0f;
-        float w = 0.0f;
-        if (in && t >= 0.0f && t < (float)(p.n - 1)) {
-            const float g = p.g[k * (p.n - 1) + (int)t], total = p.total[k * p.n + i];
-            if (g != 0.0f) {
-                w = g / total;
-                if (!(total >= kSmall) || !(fabsf(w) < kInf)) { w = 0.0f; any_redo = true; }
-            }
+        stage<K, G>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
+#pragma unroll
+        for (int x = lane; x < kTile * kWaveRows<G>; x += 64) {
+            const Step s = step_of(q0 + x / kWaveRows<G>, w.r0 + x % kWaveRows<G>, false);
+            const bool redo = unseen(s);
+            any_redo |= redo;
+            reinterpret_cast<float*>(when[w.wave])[x] = s.t;
+            reinterpret_cast<float*>(weight[w.wave])[x] = redo || s.g == 0.0f ? 0.0f : s.g / s.total;
         }
-        reinterpret_cast<float*>(when[wave])[lane] = t;
-        reinterpret_cast<float*>(weight[wave])[lane] = w;
         __syncthreads();
-        for (int qq = 0; qq < count; ++qq) {
-            const float4 tt = when[wave][qq], ww = weight[wave][qq];
-            const float* at = tile + qq * 64 * K;
+        for (int q = 0; q < count; ++q) {
+            const float4 tt = when[w.wave][q][w.group], ww = weight[w.wave][q][w.group];
+            const float* at = tile + q * G * K;
 #pragma unroll
             for (int x = 0; x < K; ++x) {
-                const float y = at[column<K>(x, lane)];
+                const float y = at[column<K, G>(x, l)];
                 sum[0][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.x, 0.0f, 1.0f), ww.x, sum[0][x]);
                 sum[1][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.y, 0.0f, 1.0f), ww.y, sum[1][x]);
                 sum[2][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.z, 0.0f, 1.0f), ww.z, sum[2][x]);
@@ -471,200 +614,237 @@ __global__ __launch_bounds__(64 * kWaves) void k_shared_grad(LogpParams p)
             }
         }
     }
-    const uint64_t redo = __ballot(any_redo);
-    __syncthreads();
     Row<E, K> raw[kRows];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) load_row<E, K>(row0 + (int64_t)min(r0 + r, p.n - 1) * p.row_stride, lane, cols, raw[r]);
+    for (int r = 0; r < kRows; ++r)
+        load_row<E, K, G>(row0 + (int64_t)min(w.mine + r, p.n - 1) * p.row_stride, l, w.cols, raw[r]);
+    // + g at the chosen entries, through LDS: a row of zeros, the choices of 16 tours added with equal ones joined first
+    // (all lanes then write different entries), further tours after them in their order.
+    const bool once = G == 64 && p.per <= 16;           // 16 lanes a row: the four rows' choices at one go
+    Step mine{};
+    bool redo_mine = false;
+    if (once) {
+        mine = step_of(lane & 15, w.mine + (lane >> 4), true);
+        redo_mine = unseen(mine);
+        join_equal(mine.to, mine.g);
+    }
+    const bool redo_any = __any(any_redo);
+    __syncthreads();
+    float* const hits = tile + (w.wave * (64 / G) + w.group) * G * K;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-        const int ii = r0 + r;
-        if (ii >= p.n) break;
-        const E* row = row0 + (int64_t)ii * p.row_stride;
+        const int i = w.mine + r;
+        if (G == 64 && i >= p.n) break;
         float h[K], d[K];
-        end_row<E, K>(raw[r], lane, cols, h);
-        const float from = base_of(p.top[map * p.n + ii]);
+        end_row<E, K, G>(raw[r], l, w.cols, h);
+        const float from = base_of(p.top[w.map * p.n + min(i, p.n - 1)]);
         // an entry that no tour had open may hold anything: its weight is 0, and so is its gradient
 #pragma unroll
-        for (int x = 0; x < K; ++x)
-            d[x] = sum[r][x] != 0.0f ? -sum[r][x] * scaled_exp(h[x] - from) : 0.0f;
-        // + g at the chosen entries.  Tours of one map often choose the same one: they are added one after the other,
-        // in their order, by one lane at a time.
+        for (int x = 0; x < K; ++x) d[x] = sum[r][x] != 0.0f ? -sum[r][x] * scaled_exp(h[x] - from) : 0.0f;
 #pragma unroll
-        for (int x = 0; x < K; ++x) hits[column<K>(x, lane)] = 0.0f;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // the lanes of a wave write each other's columns
-        const bool row_redo = redo & (0x1111111111111111ull << r);
-        for (int q0 = 0; q0 < p.per; q0 += 64) {
-            const int q = q0 + lane;
-            const int64_t k = map * p.per + q;
-            float g = 0.0f;
-            int to = -1;
-            bool again = false;
-            float t = 0.0f;
-            if (q < p.per) {
-                t = p.pos[k * p.n + ii];
-                if (t >= 0.0f && t < (float)(p.n - 1)) {
-                    g = p.g[k * (p.n - 1) + (int)t];
-                    const float total = p.total[k * p.n + ii];
-                    again = g != 0.0f && (!(total >= kSmall) || !(fabsf(g / total) < kInf));
-                    to = (int)p.next[k * p.n + ii] - col0;
-                }
+        for (int x = 0; x < K; ++x) hits[column<K, G>(x, l)] = 0.0f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the lanes of a group write each other's columns
+        constexpr int at_once = G == 64 ? 64 : 16;
+        for (int q0 = 0; q0 < p.per; q0 += at_once) {
+            Step s;
+            if (once) {
+                s = mine;
+                if ((lane >> 4) != r) s.to = -1;
+            } else {
+                s = step_of(q0 + (G == 64 ? lane : l), i, true);
             }
-            if (row_redo) {
-                uint64_t todo = __ballot(again);
-                while (todo) {
-                    const int l = __ffsll((unsigned long long)todo) - 1;
-                    todo &= todo - 1;
-                    const int64_t kk = map * p.per + q0 + l;
-                    const float tt = lane_value(t, l), gg = lane_value(g, l);
-                    float m, s;
-                    open_sum<E, K>(row - col0, p.pos + kk * p.n, tt, p.n, lane, m, s);
-                    if (s == 0.0f) {                    // nothing was open: no choice, no gradient
-                        if (lane == l) to = -1;
-                        continue;
-                    }
-                    const float ws = gg / s;
+            if (redo_any) {
+                const bool todo = once ? redo_mine && (lane >> 4) == r : unseen(s);
+                const Step own = once ? step_of(lane & 15, w.mine + (lane >> 4), false) : s;
+                for (Turns<G> turns(todo, lane); turns.more();) {
+                    const int turn = turns.take(), src = max(turn, 0);
+                    const int q = q0 + (once || G == 16 ? src & 15 : src);
+                    const float tt = __shfl(own.t, src), gg = __shfl(own.g, src);
+                    if (turn < 0) continue;
+                    const float* pos = p.pos + (w.map * p.per + q) * (int64_t)p.n;
+                    float m, total;
+                    open_sum<E, K, G>(row0 - w.col0 + (int64_t)i * p.row_stride, pos, tt, p.n, l, m, total);
+                    const float ws = gg / total;
 #pragma unroll
                     for (int x = 0; x < K; ++x) {
-                        const int j = column<K>(x, lane);
-                        if (j < cols && p.pos[kk * p.n + col0 + j] > tt)
-                            d[x] -= ws * __builtin_amdgcn_exp2f((h[x] - base_of(m)) * kLog2e);
+                        const int j = column<K, G>(x, l);
+                        if (j < w.cols && pos[w.col0 + j] > tt) d[x] -= ws * plain_exp(h[x] - base_of(m));
                     }
                 }
             }
-            uint64_t chosen = __ballot(g != 0.0f && to >= 0 && to < cols);
-            while (chosen) {
-                const int l = __ffsll((unsigned long long)chosen) - 1;
-                chosen &= chosen - 1;
-                if (lane == l) __hip_atomic_fetch_add(&hits[to], g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-            }
+            if (!once) join_equal(s.to, s.g);
+            const bool hit = s.to >= 0 && s.to < w.cols;
+#pragma unroll
+            for (int c = 0; c < (G == 64 ? 4 : 1); ++c)
+                if (hit && (G == 16 || (lane >> 4) == c))
+                    __hip_atomic_fetch_add(&hits[s.to], s.g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int x = 0; x < K; ++x) d[x] += hits[column<K>(x, lane)];
+        for (int x = 0; x < K; ++x) d[x] += hits[column<K, G>(x, l)];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        store_row<E, K>(static_cast<E*>(p.grad) + (map * p.n + ii) * (int64_t)p.n + col0, lane, cols, d);
+        if (G == 64 || i < p.n)
+            store_row<E, K, G>(static_cast<E*>(p.grad) + (w.map * p.n + i) * (int64_t)p.n + w.col0, l, w.cols, d);
     }
 }
 
-// ---- one tour a row
-template <typename E, int K>
+// ---- one tour a row: a wave has kSingleRows rows of a tour, 64 / G side by side
+template <int K, int G>
+struct SingleWork {
+    int lane, l, group, part, r0, count, col0, cols;
+    int64_t k;
+    __device__ explicit SingleWork(const LogpParams& p)
+    {
+        lane = threadIdx.x & 63;
+        l = lane & (G - 1);
+        group = lane / G;
+        const int64_t w = work_block() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), block = w / p.parts;
+        part = (int)(w % p.parts);
+        k = block / p.groups;
+        r0 = (int)(block % p.groups) * kSingleRows;
+        count = min(kSingleRows, p.rows - r0);
+        col0 = part * G * K;
+        cols = min(G * K, p.n - col0);
+    }
+};
+
+template <typename E, int K, int G>
 __global__ __launch_bounds__(256) void k_single(LogpParams p)
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t w = work_block() * 4 + wave;
-    const int part = (int)(w % p.parts);
-    const int64_t group = w / p.parts, k = group / p.groups;
-    if (k >= p.maps) return;
-    const int r0 = (int)(group % p.groups) * kSingleRows;
-    const int col0 = part * 64 * K, cols = min(64 * K, p.n - col0);
+    const SingleWork<K, G> w(p);
+    if (w.k >= p.maps) return;
+    const int lane = w.lane, l = w.l;
     const bool odd = lane & 1, high = lane & 2;
-    float pos[K];
+    const float* const at = p.pos + w.k * p.n;
+    const E* row0 = static_cast<const E*>(p.logits) + w.k * p.map_stride + (int64_t)w.r0 * p.row_stride + w.col0;
+    Row<float, K> raw_pos;
+    load_row<float, K, G>(at + w.col0, l, w.cols, raw_pos);
+    // the row whose results this lane ends up with, of four lanes each
+    const int mine = G == 64 ? 4 * (lane >> 4) + (lane & 3) : 4 * (lane & 3) + (lane >> 4);
+    const bool writes = mine < w.count && ((lane >> 2) & 3) == 0;
+    const int r_mine = w.r0 + min(mine, w.count - 1);
+    const float when = p.by_step ? (float)r_mine : at[r_mine];
+    float pos[K], top = -kInf, total = 0.0f;
+    end_row<float, K, G>(raw_pos, l, w.cols, pos);
+    if constexpr (G == 64) {
+        float z0 = 0.0f, z1 = 0.0f, z2 = 0.0f, z3 = 0.0f;
+        for (int a = 0; a < kSingleRows / 4; ++a) {
+            z0 = z1; z1 = z2; z2 = z3; z3 = 0.0f;
+            if (4 * a >= w.count) continue;
+            float h[4][K], s[4];
+            Row<E, K> raw[4];
 #pragma unroll
-    for (int x = 0; x < K; ++x) {
-        const int j = column<K>(x, lane);
-        pos[x] = j < cols ? p.pos[k * p.n + col0 + j] : -1.0f;
-    }
-    const int count = min(kSingleRows, p.rows - r0);
-    const int mine = 4 * (lane >> 4) + (lane & 3);      // the row whose results this lane ends up with
-    const int r_mine = r0 + min(mine, count - 1);
-    const float when = p.by_step ? (float)r_mine : p.pos[k * p.n + r_mine];
-    const E* row0 = static_cast<const E*>(p.logits) + k * p.map_stride + col0;
-    float z0 = 0.0f, z1 = 0.0f, z2 = 0.0f, z3 = 0.0f, top = -kInf;
-    for (int a = 0; a < kSingleRows / 4; ++a) {
-        z0 = z1; z1 = z2; z2 = z3; z3 = 0.0f;
-        if (4 * a >= count) continue;
-        float h[4][K], s[4], tt[4];
-        Row<E, K> raw[4];
+            for (int r = 0; r < 4; ++r)
+                load_row<E, K, G>(row0 + (int64_t)min(4 * a + r, w.count - 1) * p.row_stride, l, w.cols, raw[r]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = min(4 * a + r, count - 1);
-            load_row<E, K>(row0 + (int64_t)(r0 + i) * p.row_stride, lane, cols, raw[r]);
-            tt[r] = lane_value(when, 16 * (i >> 2) + (i & 3));
-        }
+            for (int r = 0; r < 4; ++r) {
+                const float tt = lane_value(when, 16 * a + r);
+                end_row<E, K, G>(raw[r], l, w.cols, h[r]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float m = -kInf;
-            end_row<E, K>(raw[r], lane, cols, h[r]);
-#pragma unroll
-            for (int x = 0; x < K; ++x) {
-                h[r][x] = pos[x] > tt[r] ? h[r][x] : -kInf;
-                m = fmaxf(m, h[r][x]);
+                for (int x = 0; x < K; ++x) h[r][x] = pos[x] > tt ? h[r][x] : -kInf;
+                s[r] = max_of(h[r]);
             }
-            m = row_max(m);
-            const float from = base_of(m);
-            float sum = 0.0f;
+            float m = quads(s, odd, high, Max());
+            m = swap32(swap16(m, m, Max()), swap16(m, m, Max()), Max());
+            top = (lane >> 4) == a ? m : top;
 #pragma unroll
-            for (int x = 0; x < K; ++x) sum += __builtin_amdgcn_exp2f((h[r][x] - from) * kLog2e);
-            s[r] = sum;
-            top = mine == 4 * a + r ? m : top;
+            for (int r = 0; r < 4; ++r) {
+                const float from = base_of(lane_value(m, r));
+                s[r] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < K; ++x) s[r] += plain_exp(h[r][x] - from);
+            }
+            z3 = quads(s, odd, high, Add());
         }
-        z3 = quad_sum(s, odd, high);
+        total = rows_sum(z0, z1, z2, z3);
+    } else {
+        constexpr int U = K > 8 ? 2 : 4;                // rows of a group in flight
+#pragma unroll
+        for (int a0 = 0; a0 < 4; a0 += U) {
+            Row<E, K> raw[U];
+            float tt[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = min(4 * (a0 + u) + w.group, w.count - 1);
+                load_row<E, K, G>(row0 + (int64_t)r * p.row_stride, l, w.cols, raw[u]);
+                tt[u] = p.by_step ? (float)(w.r0 + r) : at[w.r0 + r];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float h[K], s = 0.0f;
+                end_row<E, K, G>(raw[u], l, w.cols, h);
+#pragma unroll
+                for (int x = 0; x < K; ++x) h[x] = pos[x] > tt[u] ? h[x] : -kInf;
+                const float m = all<G>(max_of(h), Max()), from = base_of(m);
+#pragma unroll
+                for (int x = 0; x < K; ++x) s += plain_exp(h[x] - from);
+                s = all<G>(s, Add());
+                const bool own = (lane & 3) == a0 + u;
+                top = own ? m : top;
+                total = own ? s : total;
+            }
+        }
     }
-    const float total = rows_sum(z0, z1, z2, z3);
-    const bool writes = mine < count && ((lane >> 2) & 3) == 0;
-    const int64_t at = k * p.rows + r0 + mine;
+    const int64_t to = w.k * p.rows + w.r0 + mine;
     if (writes) {
-        (p.parts == 1 ? p.top : p.part_top + (int64_t)part * p.maps * p.rows)[at] = top;
-        (p.parts == 1 ? p.total : p.part_total + (int64_t)part * p.maps * p.rows)[at] = total;
+        (p.parts == 1 ? p.top : p.part_top + (int64_t)w.part * p.maps * p.rows)[to] = top;
+        (p.parts == 1 ? p.total : p.part_total + (int64_t)w.part * p.maps * p.rows)[to] = total;
     }
     if (p.parts == 1)
-        end_steps<E, K, false>(p, writes && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), k, k, r0 + mine, when, top,
-                            total, lane);
+        end_steps<E, K, G, false>(p, writes && at[0] >= 0.0f && when < (float)(p.n - 1), w.k, w.k, w.r0 + mine, when, top,
+                                  total, lane);
 }
 
-template <typename E, int K>
+template <typename E, int K, int G>
 __global__ __launch_bounds__(256) void k_single_grad(LogpParams p)
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t w = work_block() * 4 + wave;
-    const int part = (int)(w % p.parts);
-    const int64_t group = w / p.parts, k = group / p.groups;
-    if (k >= p.maps) return;
-    const int r0 = (int)(group % p.groups) * kSingleRows;
-    const int col0 = part * 64 * K, cols = min(64 * K, p.n - col0);
-    float pos[K];
-#pragma unroll
-    for (int x = 0; x < K; ++x) {
-        const int j = column<K>(x, lane);
-        pos[x] = j < cols ? p.pos[k * p.n + col0 + j] : -1.0f;
-    }
-    const int count = min(kSingleRows, p.rows - r0);
+    const SingleWork<K, G> w(p);
+    if (w.k >= p.maps) return;
+    const int lane = w.lane, l = w.l;
+    const float* const at = p.pos + w.k * p.n;
+    const E* row0 = static_cast<const E*>(p.logits) + w.k * p.map_stride + (int64_t)w.r0 * p.row_stride + w.col0;
+    E* out0 = static_cast<E*>(p.grad) + (w.k * p.rows + w.r0) * (int64_t)p.n + w.col0;
+    Row<float, K> raw_pos;
+    load_row<float, K, G>(at + w.col0, l, w.cols, raw_pos);
     float when = 0.0f, from = 0.0f, weight = 0.0f, g = 0.0f;        // of row r0 + lane
-    if (lane < count) {
-        const int64_t at = k * p.rows + r0 + lane;
-        when = p.by_step ? (float)(r0 + lane) : p.pos[k * p.n + r0 + lane];
-        from = base_of(p.top[at]);
-        const float total = p.total[at];
-        if (p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1) && total != 0.0f) {
-            g = p.g[k * (p.n - 1) + (int)when];
-            weight = g / total;
+    if (lane < w.count) {
+        const int64_t row = w.k * p.rows + w.r0 + lane;
+        when = p.by_step ? (float)(w.r0 + lane) : at[w.r0 + lane];
+        from = base_of(p.top[row]);
+        const float total = p.total[row];
+        if (at[0] >= 0.0f && when < (float)(p.n - 1) && total != 0.0f) {
+            g = p.g[w.k * (p.n - 1) + (int)when];
+            weight = -g / total;
         }
     }
-    const E* row0 = static_cast<const E*>(p.logits) + k * p.map_stride + r0 * p.row_stride + col0;
-    E* out0 = static_cast<E*>(p.grad) + (k * p.rows + r0) * (int64_t)p.n + col0;
-    for (int r0 = 0; r0 < count; r0 += 2) {             // two rows in flight
-        Row<E, K> raw[2];
+    float pos[K];
+    end_row<float, K, G>(raw_pos, l, w.cols, pos);
+    constexpr int side = 64 / G, U = G == 64 ? 2 : K > 8 ? 2 : 4;   // rows side by side, and in flight of each
+    for (int a = 0; a < w.count; a += side * U) {
+        Row<E, K> raw[U];
 #pragma unroll
-        for (int a = 0; a < 2; ++a) load_row<E, K>(row0 + (int64_t)min(r0 + a, count - 1) * p.row_stride, lane, cols, raw[a]);
+        for (int u = 0; u < U; ++u)
+            load_row<E, K, G>(row0 + (int64_t)min(a + u * side + w.group, w.count - 1) * p.row_stride, l, w.cols, raw[u]);
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const int r = r0 + a;
-            if (r >= count) break;
-            const float tt = lane_value(when, r), ff = lane_value(from, r), ww = lane_value(weight, r), gg = lane_value(g, r);
-            float d[K];
-            end_row<E, K>(raw[a], lane, cols, d);
-            if (gg == 0.0f) {                           // whatever the row holds
-#pragma unroll
-                for (int x = 0; x < K; ++x) d[x] = 0.0f;
+        for (int u = 0; u < U; ++u) {
+            const int r = a + u * side + w.group;
+            if (a + u * side >= w.count) break;
+            float tt, ff, ww, gg, d[K];
+            if constexpr (G == 64) {
+                tt = lane_value(when, r); ff = lane_value(from, r); ww = lane_value(weight, r); gg = lane_value(g, r);
             } else {
-#pragma unroll
-                for (int x = 0; x < K; ++x) {
-                    const float y = -ww * __builtin_amdgcn_exp2f((d[x] - ff) * kLog2e);
-                    d[x] = pos[x] > tt ? (pos[x] == tt + 1.0f ? y + gg : y) : 0.0f;
-                }
+                tt = __shfl(when, r); ff = __shfl(from, r); ww = __shfl(weight, r); gg = __shfl(g, r);
             }
-            store_row<E, K>(out0 + (int64_t)r * p.n, lane, cols, d);
+            end_row<E, K, G>(raw[u], l, w.cols, d);
+            const bool none = gg == 0.0f;               // then whatever the row holds
+            tt = none ? 65536.0f : tt;
+            const float chosen = tt + 1.0f;
+#pragma unroll
+            for (int x = 0; x < K; ++x) {
+                const float y = ww * plain_exp(d[x] - ff);
+                d[x] = pos[x] > tt ? (pos[x] == chosen ? y + gg : y) : 0.0f;
+            }
+            if (G == 64 || r < w.count) store_row<E, K, G>(out0 + (int64_t)r * p.n, l, w.cols, d);
         }
     }
 }
@@ -674,36 +854,36 @@ template <typename E, bool SHARED>
 __global__ __launch_bounds__(256) void k_join(LogpParams p)
 {
     const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x, all = p.maps * p.per * p.rows;
-    const bool in = w < all;
-    const int64_t k = in ? w / p.rows : 0;
+    const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x, every = p.maps * p.per * p.rows;
+    const bool in = w < every;
+    const int64_t k = in ? w / p.rows : 0, map = SHARED ? k / p.per : k;
     const int r = in ? (int)(w - k * p.rows) : 0;
-    const int64_t row = SHARED ? k / p.per * p.rows + r : w;
+    const int64_t row = map * p.rows + r;
     float top = -kInf, total = 0.0f;
     if (in) {
-        for (int c = 0; c < p.parts; ++c) top = fmaxf(top, p.part_top[c * p.maps * p.rows + row]);
+        for (int c = 0; c < p.parts; ++c) top = vmax(top, p.part_top[c * p.maps * p.rows + row]);
         for (int c = 0; c < p.parts; ++c) {
-            const float m = base_of(p.part_top[c * p.maps * p.rows + row]), s = p.part_total[c * all + w];
+            const float m = base_of(p.part_top[c * p.maps * p.rows + row]), s = p.part_total[c * every + w];
             const float x = (m - base_of(top)) * kLog2e;
             if (s == 0.0f) continue;
             // a shared sum is up to 2^76 and counts down to 2^-80: its factor must not be flushed before it is applied
             total += SHARED && x < -40.0f ? s * __builtin_amdgcn_exp2f(x + 60.0f) * (1.0f / kScale)
                                           : s * __builtin_amdgcn_exp2f(x);
         }
-        p.total[w] = total;
         if (!SHARED || k % p.per == 0) p.top[row] = top;
     }
     const float when = in ? (p.by_step ? (float)r : p.pos[k * p.n + r]) : 0.0f;
-    end_steps<E, kMaxPer, SHARED>(p, in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), SHARED ? k / p.per : k, k, r, when,
-                         top, total, lane);
+    total = end_steps<E, kMaxPer, 64, SHARED>(p, in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), map, k, r, when,
+                                              top, total, lane);
+    if (in) p.total[w] = total;
 }
 
-// Columns of a wave: the fewest registers a lane that hold the row, or an even part of a long one.
+// Columns of a group of lanes: the fewest registers a lane that hold the row, or an even part of a long one.
 inline int parts_of(int n) { return (n + 64 * kMaxPer - 1) / (64 * kMaxPer); }
 
 inline int held(int n)
 {
-    const int parts = parts_of(n), need = ((n + parts - 1) / parts + 63) / 64;
+    const int lanes = n <= kShortRow ? 16 : 64, parts = parts_of(n), need = ((n + parts - 1) / parts + lanes - 1) / lanes;
     for (int k : {1, 2, 4, 6, 8, 12})
         if (need <= k) return k;
     return kMaxPer;
@@ -721,39 +901,44 @@ inline int held(int n)
     }
 
 template <typename Kernel>
-int shared_launch(Kernel kern, LogpParams p, unsigned grid, size_t lds, hipStream_t stream)
+int logp_start(Kernel kern, LogpParams p, int64_t grid, int threads, size_t lds, hipStream_t stream)
 {
+    if (grid > 0x7fffffffll) return fail(TSP2OPT_E_UNSUPPORTED, "too many rows");
     if (lds > 48 * 1024)
         HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                     (int)lds));
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kWaves), lds, stream, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), lds, stream, p);
     return 0;
+}
+
+template <typename E, int K, int G>
+int logp_rows(LogpParams p, bool grad, hipStream_t stream)
+{
+    if (p.per > 1) {
+        constexpr int per_block = kWaves<G> * kWaveRows<G>;
+        const int tours = p.per < kTile ? p.per : kTile, words = grad && tours * G < kWaves<G> * 64 ? kWaves<G> * 64 : tours * G;
+        p.groups = (p.rows + per_block - 1) / per_block;
+        return logp_start(grad ? k_shared_grad<E, K, G> : k_shared<E, K, G>, p, p.maps * p.groups * p.parts,
+                          64 * kWaves<G>, sizeof(float) * K * words, stream);
+    }
+    p.groups = (p.rows + kSingleRows - 1) / kSingleRows;
+    return logp_start(grad ? k_single_grad<E, K, G> : k_single<E, K, G>, p, (p.maps * p.groups * p.parts + 3) / 4, 256, 0,
+                      stream);
 }
 
 template <typename E>
 int logp_launch(LogpParams p, bool grad, hipStream_t stream)
 {
-    const bool shared = p.per > 1;
-    const int k = held(p.n), per_block = shared ? kWaves * kRows : kSingleRows;
     p.parts = parts_of(p.n);
-    p.groups = (p.rows + per_block - 1) / per_block;
-    p.tile = p.per < kTile ? p.per : kTile;
-    const int64_t units = p.maps * p.groups * p.parts, grid = shared ? units : (units + 3) / 4;
-    if (grid > 0x7fffffffll) return fail(TSP2OPT_E_UNSUPPORTED, "too many rows");
+    const int k = held(p.n);
     int rc = 0;
-    if (shared) {
-        const size_t lds = sizeof(float) * 64 * k * (grad && p.tile < kWaves ? kWaves : p.tile);
-        if (grad) T2O_BY_HELD(k, (rc = shared_launch(k_shared_grad<E, K>, p, (unsigned)grid, lds, stream)))
-        else T2O_BY_HELD(k, (rc = shared_launch(k_shared<E, K>, p, (unsigned)grid, lds, stream)))
-    } else {
-        if (grad) T2O_BY_HELD(k, hipLaunchKernelGGL((k_single_grad<E, K>), dim3((unsigned)grid), dim3(256), 0, stream, p))
-        else T2O_BY_HELD(k, hipLaunchKernelGGL((k_single<E, K>), dim3((unsigned)grid), dim3(256), 0, stream, p))
-    }
+    if (p.n <= kShortRow) T2O_BY_HELD(k, (rc = logp_rows<E, K, 16>(p, grad, stream)))
+    else T2O_BY_HELD(k, (rc = logp_rows<E, K < 6 ? 6 : K, 64>(p, grad, stream)))
     if (rc) return rc;
     if (!grad && p.parts > 1) {
-        const unsigned blocks = (unsigned)((p.maps * p.per * p.rows + 255) / 256);
-        if (shared) hipLaunchKernelGGL((k_join<E, true>), dim3(blocks), dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((k_join<E, false>), dim3(blocks), dim3(256), 0, stream, p);
+        const int64_t blocks = (p.maps * p.per * p.rows + 255) / 256;
+        rc = logp_start(p.per > 1 ? k_join<E, true> : k_join<E, false>, p, blocks, 256, 0, stream);
+        if (rc) return rc;
     }
     HIP_TRY(hipGetLastError());
     return 0;
