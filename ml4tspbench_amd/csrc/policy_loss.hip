@@ -6,11 +6,18 @@
 //     l = -(1 - eps) log sigmoid(s_a - s_b) - eps log sigmoid(s_b - s_a)
 // Both are averages; the gradients are recomputed from the same inputs in one pass.  Sums over steps and rows are
 // kept in double and added in a fixed order: results do not depend on the schedule.
+//
+// A row of steps is read by a group of G threads: 8 for short rows (eight rows a wave), a wave, or for long rows of few
+// tours a whole workgroup.  Bound by memory where there is much, by the launches and the host's autograd where there is
+// little: up to kOneBlock steps one workgroup does everything, sums and end, in one launch.
 #include "learn_common.hpp"
 
 namespace t2o {
 
-constexpr int kMaxBlocks = 1024;        // partial sums the finishing workgroup adds up
+constexpr int kMaxBlocks = 2048;        // partial sums the finishing workgroup adds up
+constexpr int kBlockRow = 1024;         // threads of a workgroup that has a row to itself
+constexpr int64_t kOneBlock = 16384;    // steps that one workgroup of kOneThreads takes in one launch
+constexpr int kOneThreads = 1024;
 constexpr int kRatioTour = 1, kAverageTour = 2;
 
 struct PolicyParams {
@@ -22,7 +29,7 @@ struct PolicyParams {
     float lo, hi;
     double kl_coef, log_lo, log_hi;
     float *loss, *stats;    // stats: kl, clip fraction
-    double* partial;        // [blocks][4]
+    double* partial;        // [blocks][4]; with one block unused
     double* norm;           // 1 / what the averages divide by
     float2* rows;           // (T): gradient of the ratio term w.r.t. a whole tour's x; 1 / kept steps
     const float* g;
@@ -54,90 +61,122 @@ __device__ __forceinline__ bool is_cut(const PolicyParams& p, float adv, double 
     return (adv > 0.0f && x > p.log_hi) || (adv < 0.0f && x < p.log_lo);
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void k_policy(PolicyParams p)
+// Sum over a group of G threads (over the workgroup where G is more than a wave), in every thread of it.
+template <int G, int N>
+__device__ __forceinline__ void group_sum(double (&v)[N])
 {
-    __shared__ double part[4][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+        for (int o = (G < 64 ? G : 64) / 2; o >= 1; o >>= 1) v[c] += __shfl_xor(v[c], o);
+    if constexpr (G > 64) {
+        __shared__ double part[G / 64][N];
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0)
+            for (int c = 0; c < N; ++c) part[threadIdx.x >> 6][c] = v[c];
+        __syncthreads();
+        for (int c = 0; c < N; ++c) {
+            double s = 0.0;
+            for (int w = 0; w < (int)blockDim.x / 64; ++w) s += part[w][c];
+            v[c] = s;
+        }
+    }
+}
+
+// The group of G threads that a thread belongs to, and how many there are.
+template <int G>
+struct Groups {
+    int64_t first, count;
+    int at;
+    __device__ Groups()
+    {
+        const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+        first = t / G;
+        count = (int64_t)gridDim.x * blockDim.x / G;
+        at = (int)(t % G);
+    }
+};
+
+__device__ __forceinline__ void policy_end(const PolicyParams& p, const double (&v)[4])
+{
+    const double inv = v[3] > 0.0 ? 1.0 / v[3] : 0.0, kl = v[1] * inv;
+    p.norm[0] = inv;
+    p.loss[0] = (float)(v[0] * inv + (p.kl_coef != 0.0 ? p.kl_coef * kl : 0.0));
+    p.stats[0] = (float)kl;
+    p.stats[1] = (float)(v[2] * inv);
+}
+
+template <typename E, int G>
+__global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
+{
+    const Groups<G> g;
     double sum[4] = {0.0, 0.0, 0.0, 0.0};               // ratio term, kl, clipped, weight
-    for (int64_t k = (int64_t)blockIdx.x * 4 + wave; k < p.T; k += (int64_t)gridDim.x * 4) {
-        const int64_t base = k * p.S;
-        double term = 0.0, kl = 0.0, clip = 0.0, count = 0.0, whole = 0.0;
-        for (int64_t s = lane; s < p.S; s += 64) {
-            const int64_t i = base + s;
+    for (int64_t k = g.first; k < p.T; k += g.count) {
+        double v[5] = {0.0, 0.0, 0.0, 0.0, 0.0};        // ratio term, kl, clipped, steps, difference of the tour
+        for (int64_t s = g.at; s < p.S; s += G) {
+            const int64_t i = k * p.S + s;
+            const float lp = widen(static_cast<const E*>(p.lp)[i]), old = widen(static_cast<const E*>(p.old)[i]);
+            const float ref = p.ref ? widen(static_cast<const E*>(p.ref)[i]) : lp;
             if (p.mask && !p.mask[i]) continue;
-            const float lp = widen(static_cast<const E*>(p.lp)[i]);
-            const double x = (double)lp - (double)widen(static_cast<const E*>(p.old)[i]);
-            count += 1.0;
+            const double x = (double)lp - (double)old;
+            v[3] += 1.0;
             if (p.mode & kRatioTour) {
-                whole += x;
+                v[4] += x;
             } else {
                 const float adv = p.adv[p.adv_per_step ? i : k];
                 const bool cut = is_cut(p, adv, x);
-                term += (double)(-adv * (cut ? (adv > 0.0f ? p.hi : p.lo) : expf((float)x)));
-                clip += cut ? 1.0 : 0.0;
+                v[0] += (double)(-adv * (cut ? (adv > 0.0f ? p.hi : p.lo) : expf((float)x)));
+                v[2] += cut ? 1.0 : 0.0;
             }
-            if (p.ref) kl += (double)kl_term(widen(static_cast<const E*>(p.ref)[i]) - lp);
+            if (p.ref) v[1] += (double)kl_term(ref - lp);
         }
         if (p.mode == 0) {
-            sum[0] += term; sum[1] += kl; sum[2] += clip; sum[3] += count;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += v[c];
             continue;
         }
-        term = wave_sum(term); kl = wave_sum(kl); clip = wave_sum(clip); count = wave_sum(count);
-        const double inv = count > 0.0 ? 1.0 / count : 0.0;
+        group_sum<G>(v);
+        const double inv = v[3] > 0.0 ? 1.0 / v[3] : 0.0;
         float c = 0.0f;
         if (p.mode & kRatioTour) {
-            whole = wave_sum(whole);
-            const float adv = p.adv[k], r = expf((float)whole);
-            const bool cut = is_cut(p, adv, whole);
-            c = cut ? 0.0f : -adv * r;
-            term = cut ? -adv * (adv > 0.0f ? p.hi : p.lo) : c;
-            clip = cut ? 1.0 : 0.0;
+            const float adv = p.adv[k];
+            const bool cut = is_cut(p, adv, v[4]);
+            c = cut ? 0.0f : -adv * expf((float)v[4]);
+            v[0] = cut ? -adv * (adv > 0.0f ? p.hi : p.lo) : c;
+            v[2] = cut ? 1.0 : 0.0;
         } else {
-            term *= inv;
-            clip *= inv;
+            v[0] *= inv;
+            v[2] *= inv;
         }
-        if (lane == 0) {
-            if (count > 0.0) { sum[0] += term; sum[1] += kl * inv; sum[2] += clip; sum[3] += 1.0; }
-            p.rows[k] = make_float2(count > 0.0 ? c : 0.0f, (float)inv);
+        if (g.at == 0) {
+            if (v[3] > 0.0) { sum[0] += v[0]; sum[1] += v[1] * inv; sum[2] += v[2]; sum[3] += 1.0; }
+            p.rows[k] = make_float2(v[3] > 0.0 ? c : 0.0f, (float)inv);
         }
     }
-    for (int c = 0; c < 4; ++c) {
-        const double v = wave_sum(sum[c]);
-        if (lane == 0) part[wave][c] = v;
-    }
-    __syncthreads();
-    if (threadIdx.x < 4)
-        p.partial[blockIdx.x * 4 + threadIdx.x] =
-            part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+    group_sum<1024>(sum);
+    if (threadIdx.x != 0) return;
+    if (gridDim.x == 1) policy_end(p, sum);
+    else
+        for (int c = 0; c < 4; ++c) p.partial[blockIdx.x * 4 + c] = sum[c];
 }
 
-__global__ __launch_bounds__(64) void k_policy_end(PolicyParams p, int blocks)
+__global__ __launch_bounds__(1024) void k_policy_end(PolicyParams p, int blocks)
 {
-    double v[4];
-    for (int c = 0; c < 4; ++c) {
-        double s = 0.0;
-        for (int b = threadIdx.x; b < blocks; b += 64) s += p.partial[b * 4 + c];
-        v[c] = wave_sum(s);
-    }
-    if (threadIdx.x == 0) {
-        const double inv = v[3] > 0.0 ? 1.0 / v[3] : 0.0;
-        p.norm[0] = inv;
-        const double kl = v[1] * inv;
-        p.loss[0] = (float)(v[0] * inv + (p.kl_coef != 0.0 ? p.kl_coef * kl : 0.0));
-        p.stats[0] = (float)kl;
-        p.stats[1] = (float)(v[2] * inv);
-    }
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int b = threadIdx.x; b < blocks; b += 1024)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] += p.partial[b * 4 + c];
+    group_sum<1024>(v);
+    if (threadIdx.x == 0) policy_end(p, v);
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void k_policy_grad(PolicyParams p)
+template <typename E, int G>
+__global__ __launch_bounds__(1024) void k_policy_grad(PolicyParams p)
 {
-    const int lane = threadIdx.x & 63;
+    const Groups<G> g;
     const float scale = (float)(p.norm[0] * (double)p.g[0]);
-    for (int64_t k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); k < p.T; k += (int64_t)gridDim.x * 4) {
+    for (int64_t k = g.first; k < p.T; k += g.count) {
         const float2 row = p.mode ? p.rows[k] : make_float2(0.0f, 1.0f);
-        for (int64_t s = lane; s < p.S; s += 64) {
+        for (int64_t s = g.at; s < p.S; s += G) {
             const int64_t i = k * p.S + s;
             float d = 0.0f;
             if (!p.mask || p.mask[i]) {
@@ -179,106 +218,121 @@ struct PrefParams {
     void* grad;
 };
 
-template <typename E>
-__global__ __launch_bounds__(256) void k_pref_rows(PrefParams p)
+template <typename E, int G>
+__device__ __forceinline__ void pref_rows(const PrefParams& p)
 {
-    const int lane = threadIdx.x & 63;
-    for (int64_t k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); k < p.T; k += (int64_t)gridDim.x * 4) {
-        double x = 0.0, count = 0.0;
-        for (int64_t s = lane; s < p.S; s += 64) {
+    const Groups<G> g;
+    for (int64_t k = g.first; k < p.T; k += g.count) {
+        double v[2] = {0.0, 0.0};                       // sum, steps
+        for (int64_t s = g.at; s < p.S; s += G) {
             const int64_t i = k * p.S + s;
+            const double lp = (double)widen(static_cast<const E*>(p.lp)[i]);
+            const double ref = p.ref ? (double)widen(static_cast<const E*>(p.ref)[i]) : 0.0;
             if (p.mask && !p.mask[i]) continue;
-            double v = (double)widen(static_cast<const E*>(p.lp)[i]);
-            if (p.ref) v -= (double)widen(static_cast<const E*>(p.ref)[i]);
-            x += v;
-            count += 1.0;
+            v[0] += lp - ref;
+            v[1] += 1.0;
         }
-        x = wave_sum(x);
-        count = wave_sum(count);
-        if (lane == 0) {
-            const double scale = p.per_step ? p.beta / fmax(count, 1.0) : p.beta;
-            p.score[k] = x * scale;
+        group_sum<G>(v);
+        if (g.at == 0) {
+            const double scale = p.per_step ? p.beta / fmax(v[1], 1.0) : p.beta;
+            p.score[k] = v[0] * scale;
             p.scale[k] = (float)scale;
         }
     }
 }
 
-// One workgroup an instance and 256 of its tours a; every thread walks the other tours b.
-__global__ __launch_bounds__(256) void k_pref_pairs(PrefParams p)
+// W threads a tour a walk the other tours b of its instance; loss and pairs are added up at the winner.
+template <int W>
+__device__ __forceinline__ void pref_pairs(const PrefParams& p, double (&sum)[2])
 {
-    __shared__ double sc[256], ln[256], part[4][2];
-    __shared__ int first;
-    const int64_t inst = p.T / p.per;
-    const int chunks = (p.per + 255) / 256;
-    double loss = 0.0, count = 0.0;
-    for (int64_t w = blockIdx.x; w < inst * chunks; w += gridDim.x) {
-        const int64_t base = (w / chunks) * p.per;
-        const int a = (int)(w % chunks) * 256 + threadIdx.x;
-        if (p.best && threadIdx.x == 0) {
-            int f = -1;
-            for (int b = 0; b < p.per; ++b)
-                if (p.len[base + b] == p.len[base + b] && (f < 0 || p.len[base + b] < p.len[base + f])) f = b;
-            first = f;
-        }
-        const bool in = a < p.per;
-        const double sa = in ? p.score[base + a] : 0.0, la = in ? p.len[base + a] : 0.0;
-        double c = 0.0;
-        for (int b0 = 0; b0 < p.per; b0 += 256) {
-            __syncthreads();
-            if (b0 + (int)threadIdx.x < p.per) {
-                sc[threadIdx.x] = p.score[base + b0 + threadIdx.x];
-                ln[threadIdx.x] = p.len[base + b0 + threadIdx.x];
+    const Groups<W> g;
+    for (int64_t k = g.first; k < p.T; k += g.count) {
+        const int64_t base = k / p.per * p.per;
+        const int a = (int)(k - base);
+        const double sa = p.score[k], la = p.len[k];
+        int first = -1;
+        if (p.best) {                                   // the first of the shortest; NaN is none
+            double least = 0.0;
+            for (int b = g.at; b < p.per; b += W) {
+                const double l = p.len[base + b];
+                if (l == l && (first < 0 || l < least)) { first = b; least = l; }
             }
-            __syncthreads();
-            if (!in) continue;
-            for (int q = 0; q < min(256, p.per - b0); ++q) {
-                const bool wins = la < ln[q] && (!p.best || a == first);
-                const bool loses = ln[q] < la && (!p.best || b0 + q == first);
-                if (!wins && !loses) continue;
-                const float z = (float)(wins ? sa - sc[q] : sc[q] - sa);
-                const float e = expf(-fabsf(z));
-                const float against = z >= 0.0f ? e / (1.0f + e) : 1.0f / (1.0f + e);       // sigmoid(-z)
-                c += (double)(wins ? p.eps - against : against - p.eps);
-                if (wins) {
-                    loss += (double)(fmaxf(-z, 0.0f) + log1pf(e) + (p.eps != 0.0f ? p.eps * z : 0.0f));
-                    count += 1.0;
-                }
+            for (int o = W / 2; o >= 1; o >>= 1) {
+                const int other = __shfl_xor(first, o);
+                const double l = __shfl_xor(least, o);
+                if (other >= 0 && (first < 0 || l < least || (l == least && other < first))) { first = other; least = l; }
             }
         }
-        if (in) p.coef[base + a] = (float)c;
-        __syncthreads();
+        double c[1] = {0.0};
+        for (int b = g.at; b < p.per; b += W) {
+            const double sb = p.score[base + b], lb = p.len[base + b];
+            const bool wins = la < lb && (!p.best || a == first);
+            const bool loses = lb < la && (!p.best || b == first);
+            if (!wins && !loses) continue;
+            const float z = (float)(wins ? sa - sb : sb - sa);
+            const float e = expf(-fabsf(z));
+            const float against = z >= 0.0f ? e / (1.0f + e) : 1.0f / (1.0f + e);       // sigmoid(-z)
+            c[0] += (double)(wins ? p.eps - against : against - p.eps);
+            if (wins) {
+                sum[0] += (double)(fmaxf(-z, 0.0f) + log1pf(e) + (p.eps != 0.0f ? p.eps * z : 0.0f));
+                sum[1] += 1.0;
+            }
+        }
+        group_sum<W>(c);
+        if (g.at == 0) p.coef[k] = (float)c[0];
     }
-    loss = wave_sum(loss);
-    count = wave_sum(count);
-    if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6][0] = loss; part[threadIdx.x >> 6][1] = count; }
-    __syncthreads();
-    if (threadIdx.x < 2)
-        p.partial[blockIdx.x * 2 + threadIdx.x] =
-            part[0][threadIdx.x] + part[1][threadIdx.x] + part[2][threadIdx.x] + part[3][threadIdx.x];
+    group_sum<1024>(sum);
 }
 
-__global__ __launch_bounds__(64) void k_pref_end(PrefParams p, int blocks)
+__device__ __forceinline__ void pref_end(const PrefParams& p, const double (&v)[2])
 {
-    double loss = 0.0, count = 0.0;
-    for (int b = threadIdx.x; b < blocks; b += 64) { loss += p.partial[2 * b]; count += p.partial[2 * b + 1]; }
-    loss = wave_sum(loss);
-    count = wave_sum(count);
-    if (threadIdx.x == 0) {
-        const double inv = count > 0.0 ? 1.0 / count : 0.0;
-        p.norm[0] = inv;
-        p.loss[0] = (float)(loss * inv);
-        p.pairs[0] = (int64_t)count;
-    }
+    const double inv = v[1] > 0.0 ? 1.0 / v[1] : 0.0;
+    p.norm[0] = inv;
+    p.loss[0] = (float)(v[0] * inv);
+    p.pairs[0] = (int64_t)v[1];
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void k_pref_grad(PrefParams p)
+template <typename E, int G>
+__global__ __launch_bounds__(1024) void k_pref_rows(PrefParams p)
 {
-    const int lane = threadIdx.x & 63;
+    pref_rows<E, G>(p);
+}
+
+template <int W>
+__global__ __launch_bounds__(1024) void k_pref_pairs(PrefParams p)
+{
+    double sum[2] = {0.0, 0.0};
+    pref_pairs<W>(p, sum);
+    if (threadIdx.x < 2) p.partial[blockIdx.x * 2 + threadIdx.x] = sum[threadIdx.x];
+}
+
+__global__ __launch_bounds__(1024) void k_pref_end(PrefParams p, int blocks)
+{
+    double v[2] = {0.0, 0.0};
+    for (int b = threadIdx.x; b < blocks; b += 1024) { v[0] += p.partial[2 * b]; v[1] += p.partial[2 * b + 1]; }
+    group_sum<1024>(v);
+    if (threadIdx.x == 0) pref_end(p, v);
+}
+
+// Everything in one workgroup: what little there is would otherwise take three launches.
+template <typename E, int G>
+__global__ __launch_bounds__(1024) void k_pref_one(PrefParams p)
+{
+    pref_rows<E, G>(p);
+    __syncthreads();                                    // the scores are read by other threads of this workgroup
+    double sum[2] = {0.0, 0.0};
+    pref_pairs<8>(p, sum);
+    if (threadIdx.x == 0) pref_end(p, sum);
+}
+
+template <typename E, int G>
+__global__ __launch_bounds__(1024) void k_pref_grad(PrefParams p)
+{
+    const Groups<G> g;
     const double scale = p.norm[0] * (double)p.g[0];
-    for (int64_t k = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); k < p.T; k += (int64_t)gridDim.x * 4) {
+    for (int64_t k = g.first; k < p.T; k += g.count) {
         const E d = narrow<E>((float)(scale * (double)p.coef[k] * (double)p.scale[k]));
-        for (int64_t s = lane; s < p.S; s += 64) {
+        for (int64_t s = g.at; s < p.S; s += G) {
             const int64_t i = k * p.S + s;
             static_cast<E*>(p.grad)[i] = !p.mask || p.mask[i] ? d : narrow<E>(0.0f);
         }
@@ -298,7 +352,28 @@ int loss_check(int64_t T, int64_t S, int32_t dtype)
 
 bool off(const void* ptr, size_t size) { return reinterpret_cast<uintptr_t>(ptr) % size != 0; }
 
-unsigned row_blocks(int64_t T) { return (unsigned)(T < 4 * kMaxBlocks ? (T + 3) / 4 : kMaxBlocks); }
+// How rows of S steps are shared out: threads a row, threads a workgroup, workgroups.
+struct Shape {
+    int group, threads;
+    unsigned grid;
+};
+
+Shape shape_of(int64_t T, int64_t S, bool one_block)
+{
+    Shape s;
+    s.group = S <= 24 ? 8 : S > 2048 && T < 2048 ? kBlockRow : 64;
+    s.threads = s.group == kBlockRow || one_block ? 1024 : 256;
+    const int64_t grid = (T * s.group + s.threads - 1) / s.threads;
+    s.grid = one_block ? 1u : (unsigned)(grid < kMaxBlocks ? grid : kMaxBlocks);
+    return s;
+}
+
+#define T2O_BY_GROUP(group, CALL)                                  \
+    switch (group) {                                               \
+        case 8: { constexpr int G = 8; CALL; break; }              \
+        case 64: { constexpr int G = 64; CALL; break; }            \
+        default: { constexpr int G = kBlockRow; CALL; break; }     \
+    }
 
 int64_t policy_state_bytes(int64_t T) { return kPartialBytes + round256(8 * T); }
 
@@ -385,9 +460,10 @@ extern "C" int tsp2opt_policy_loss(const void* logp, const void* old_logp, const
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     p.loss = loss_out;
     p.stats = stats_out;
-    const unsigned grid = row_blocks(num_tours);
-    if (grid) T2O_BY_DTYPE(dtype, hipLaunchKernelGGL(k_policy<E>, dim3(grid), dim3(256), 0, stream, p));
-    hipLaunchKernelGGL(k_policy_end, dim3(1), dim3(64), 0, stream, p, (int)grid);
+    const Shape s = shape_of(num_tours, steps, num_tours * steps <= kOneBlock && num_tours <= kOneBlock / 8);
+    T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_policy<E, G>), dim3(s.grid), dim3(s.threads), 0,
+                                                                 stream, p)));
+    if (s.grid > 1) hipLaunchKernelGGL(k_policy_end, dim3(1), dim3(1024), 0, stream, p, (int)s.grid);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -412,7 +488,9 @@ extern "C" int tsp2opt_policy_loss_grad(const void* logp, const void* old_logp, 
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     p.g = grad_loss;
     p.grad = grad_out;
-    T2O_BY_DTYPE(dtype, hipLaunchKernelGGL(k_policy_grad<E>, dim3(row_blocks(num_tours)), dim3(256), 0, stream, p));
+    const Shape s = shape_of(num_tours, steps, false);
+    T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_policy_grad<E, G>), dim3(s.grid), dim3(s.threads), 0,
+                                                                 stream, p)));
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -444,14 +522,21 @@ extern "C" int tsp2opt_preference_loss(const void* logp, const void* ref_logp, c
     p.per = tours_per_instance; p.best = best_only; p.per_step = per_step; p.beta = beta; p.eps = (float)label_smoothing;
     p.loss = loss_out; p.pairs = pairs_out;
     pref_state(p, state);
-    unsigned blocks = 0;
-    if (num_tours) {
-        const int64_t units = num_tours / tours_per_instance * ((tours_per_instance + 255) / 256);
-        blocks = (unsigned)(units < 2 * kMaxBlocks ? units : 2 * kMaxBlocks);
-        T2O_BY_DTYPE(dtype, hipLaunchKernelGGL(k_pref_rows<E>, dim3(row_blocks(num_tours)), dim3(256), 0, stream, p));
-        hipLaunchKernelGGL(k_pref_pairs, dim3(blocks), dim3(256), 0, stream, p);
+    if (num_tours * steps <= kOneBlock && num_tours <= 512 && tours_per_instance <= 64) {
+        const Shape s = shape_of(num_tours, steps, true);
+        T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_pref_one<E, G>), dim3(1), dim3(kOneThreads), 0,
+                                                                     stream, p)));
+    } else {
+        const Shape s = shape_of(num_tours, steps, false);
+        T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_pref_rows<E, G>), dim3(s.grid), dim3(s.threads), 0,
+                                                                     stream, p)));
+        const int w = tours_per_instance <= 64 ? 8 : 64;
+        const int64_t need = (num_tours * w + 255) / 256;
+        const unsigned blocks = (unsigned)(need < kMaxBlocks ? need : kMaxBlocks);
+        if (w == 8) hipLaunchKernelGGL(k_pref_pairs<8>, dim3(blocks), dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL(k_pref_pairs<64>, dim3(blocks), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL(k_pref_end, dim3(1), dim3(1024), 0, stream, p, (int)blocks);
     }
-    hipLaunchKernelGGL(k_pref_end, dim3(1), dim3(64), 0, stream, p, (int)blocks);
     HIP_TRY(hipGetLastError());
     return 0;
 }
@@ -473,7 +558,9 @@ extern "C" int tsp2opt_preference_loss_grad(const uint8_t* mask, const void* sta
     PrefParams p{};
     p.mask = mask; p.T = num_tours; p.S = steps; p.g = grad_loss; p.grad = grad_out;
     pref_state(p, const_cast<void*>(state));
-    T2O_BY_DTYPE(dtype, hipLaunchKernelGGL(k_pref_grad<E>, dim3(row_blocks(num_tours)), dim3(256), 0, stream, p));
+    const Shape s = shape_of(num_tours, steps, false);
+    T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_pref_grad<E, G>), dim3(s.grid), dim3(s.threads), 0,
+                                                                 stream, p)));
     HIP_TRY(hipGetLastError());
     return 0;
 }

@@ -183,8 +183,7 @@ __device__ __forceinline__ int column(int i, int l)
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x)
 {
-    const int i = __float_as_int(x);
-    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xf, 0xf, false));
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
 
 // fmaxf quiets its operands first; these are one instruction.  A NaN operand is left out, as fmaxf leaves it out.
@@ -279,9 +278,10 @@ __device__ __forceinline__ float scaled_exp(float x)
 __device__ __forceinline__ float plain_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // Maximum and sum over a row's open entries by a group of lanes: the steps that k_shared cannot see.
-template <typename E, int K, int G>
+template <typename E, int KK, int G>
 __device__ void open_sum(const E* row, const float* pos, float when, int n, int l, float& top, float& total)
 {
+    constexpr int K = KK > 8 ? 8 : KK;                  // fewer registers than the rows that wait meanwhile
     top = -kInf;
     total = 0.0f;
     for (int c = 0; c < n; c += G * K) {
@@ -327,31 +327,32 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int src)
     return ((int64_t)__shfl((int)(x >> 32), src) << 32) | (unsigned)__shfl((int)x, src);
 }
 
-// Ends the steps of the lanes with `valid`: (tour k, row r, step `when`).  A shared total is 2^60 times the sum; steps of
-// which it says nothing are redone one after the other by their group of lanes: all lanes have to be here.  Returns what
-// the gradient needs to know of the step.
+// Ends the steps of the lanes with `valid`: (tour k with positions `at`, row r, step `when`, node `next` chosen).  A shared
+// total is 2^60 times the sum; steps of which it says nothing are redone one after the other by their group of lanes:
+// all lanes have to be here.  Returns what the gradient needs to know of the step.
 template <typename E, int K, int G, bool SHARED>
-__device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, int r, float when,
-                                           float top, float total, int lane)
+__device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, const float* at, int r,
+                                           float when, int next, float top, float total, int lane)
 {
     const E* base = static_cast<const E*>(p.logits);
     const E* row = base + map * p.map_stride + (int64_t)r * p.row_stride;
     const int t = (int)when;
     float chosen = 0.0f, keep = total;
-    if (valid) chosen = widen(row[p.by_step ? (int)p.tours[k * (p.n + 1) + t + 1] : (int)p.next[k * p.n + r]]);
+    if (valid) chosen = widen(row[next]);
     // log(total) and not of total 2^-60 where that would leave the range of float
     float log_total = logf(!SHARED ? total : total >= 0x1p-60f ? total * (1.0f / kScale) : total);
     if (SHARED && total < 0x1p-60f) log_total -= 60.0f / kLog2e;
     if constexpr (SHARED) {
         for (Turns<G> turns(valid && !(total >= kSmall), lane); turns.more();) {
             const int turn = turns.take(), src = max(turn, 0);
-            const int64_t kk = shfl64(k, src), mm = shfl64(map, src);
+            const float* pos = reinterpret_cast<const float*>(shfl64(reinterpret_cast<int64_t>(at), src));
+            const int64_t mm = shfl64(map, src);
             const int rr = __shfl(r, src);
             const float ww = __shfl(when, src);
             float m = 0.0f, s = 0.0f;
             if (turn >= 0)
-                open_sum<E, K, G>(base + mm * p.map_stride + (int64_t)rr * p.row_stride, p.pos + kk * p.n, ww, p.n,
-                                  lane & (G - 1), m, s);
+                open_sum<E, K, G>(base + mm * p.map_stride + (int64_t)rr * p.row_stride, pos, ww, p.n, lane & (G - 1), m,
+                                  s);
             if (lane == turn) {
                 top = m;
                 total = s;
@@ -412,11 +413,68 @@ __device__ __forceinline__ void stage(float* tile, const float* pos, int count, 
     }
 }
 
+// The same from the tours themselves, for rows that fit a workgroup's tile whole (G = 16): k_positions for a pass's
+// tours, a wave a tour, with the successors.  A map's first workgroup also writes them down for the gradient.
+template <int K>
+__device__ __forceinline__ void stage_tours(const LogpParams& p, float* tile, uint16_t* after, int64_t k0, int count,
+                                            bool writes, int wave, int lane)
+{
+    constexpr int C = 16 * K, steps = (C + 63) / 64, per_wave = kTile / kWaves<16>;
+    for (int a = 0; a < per_wave; ++a) {
+        const int q = a * kWaves<16> + wave;
+        if (q >= count) break;
+        const int64_t k = k0 + q;
+        const int64_t* t = p.tours + k * (p.n + 1);
+        int node[steps], then[steps];
+#pragma unroll
+        for (int c = 0; c < steps; ++c) {
+            const int s = min(c * 64 + lane, p.n - 1);
+            const int64_t j = t[s], i = t[s + 1];
+            node[c] = j >= 0 && j < p.n ? (int)j : -1;
+            then[c] = (int)i;
+        }
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < steps; ++c) {
+            const int s = c * 64 + lane;
+            if (s >= p.n) continue;
+            if (node[c] < 0) bad = true;
+            else tile[q * C + node[c]] = (float)s;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int c = 0; c < steps; ++c) {
+            const int s = c * 64 + lane;
+            if (s < p.n && node[c] >= 0) {
+                bad |= tile[q * C + node[c]] != (float)s;       // two steps at one node: one of them sees the other's
+                after[q * C + node[c]] = (uint16_t)then[c];
+            }
+        }
+        bad = __any(bad);
+#pragma unroll
+        for (int c = 0; c < steps; ++c) {
+            const int j = c * 64 + lane;
+            if (j < C && (bad || j >= p.n)) tile[q * C + j] = j < p.n ? -1.0f : -kInf;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (!writes) continue;
+#pragma unroll
+        for (int c = 0; c < steps; ++c) {
+            const int j = c * 64 + lane;
+            if (j >= p.n) continue;
+            p.pos[k * p.n + j] = tile[q * C + j];
+            p.next[k * p.n + j] = bad ? (uint16_t)0 : after[q * C + j];
+            if (bad && j < p.n - 1) p.logp[k * (p.n - 1) + j] = __builtin_nanf("");
+        }
+    }
+}
+
 // Where a wave's work lies.
 template <int K, int G>
 struct SharedWork {
     int lane, wave, l, group, part, r0, mine, col0, cols;       // mine: first row of this lane's group of lanes
     int64_t map;
+    bool first;                                                 // the map's first workgroup
     __device__ explicit SharedWork(const LogpParams& p)
     {
         lane = threadIdx.x & 63;
@@ -426,6 +484,7 @@ struct SharedWork {
         const int64_t b = work_block(), block = b / p.parts;
         part = (int)(b % p.parts);
         map = block / p.groups;
+        first = block % p.groups == 0;
         r0 = (int)(block % p.groups) * (kWaves<G> * kWaveRows<G>) + wave * kWaveRows<G>;
         mine = r0 + group * kRows;
         col0 = part * G * K;
@@ -433,13 +492,16 @@ struct SharedWork {
     }
 };
 
-// Bound by its vector instructions: 2 K kRows for the masked additions of a tour, 11 to sum them over 16 lanes (and 2/16
-// of two swaps and an add across), an exponential and 10 more an entry of a row.
+// Bound by its vector instructions: 2 K kRows for the masked additions of a tour, 12 to sum them over the lanes, an
+// exponential and 8 more an entry of a row.  (Summing over the lanes on the matrix pipe, one v_mfma_f32_16x16x4 a row and
+// tour, takes 10 vector instructions a tour less and 13 us more on 128 maps x 16 tours of 500 nodes: it does not run
+// beside the vector pipe.)
 template <typename E, int K, int G>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 {
     extern __shared__ float tile[];                     // [tours of a pass][G K] positions
     __shared__ float4 when[kWaves<G>][kTile][64 / G];   // the steps at which the tours leave a wave's rows
+    __shared__ uint16_t after[G == 16 ? kTile * 16 * K : 1];
     const SharedWork<K, G> w(p);
     const int lane = w.lane, l = w.l;
     const bool odd = lane & 1, high = lane & 2;
@@ -450,7 +512,13 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
         load_row<E, K, G>(row0 + (int64_t)min(w.mine + r, p.n - 1) * p.row_stride, l, w.cols, raw[r]);
-    stage<K, G>(tile, p.pos + w.map * p.per * (int64_t)p.n, min(kTile, p.per), p.n, w.col0, w.cols, w.wave, lane);
+    auto stage_pass = [&](int q0, int count) {
+        if constexpr (G == 16)
+            stage_tours<K>(p, tile, after, w.map * p.per + q0, count, w.first, w.wave, lane);
+        else
+            stage<K, G>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
+    };
+    stage_pass(0, min(kTile, p.per));
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         end_row<E, K, G>(raw[r], l, w.cols, e[r]);
@@ -487,8 +555,16 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
         const float t = when_of[q * kWaveRows<G> + w.group * kRows + (lane & 3)];
         const bool in = q < count && i < p.n;
         const int64_t k = w.map * p.per + q0 + q;
-        if (p.parts == 1)
-            total = end_steps<E, K, G, true>(p, in && t >= 0.0f && t < (float)(p.n - 1), w.map, k, i, t, mine, total, lane);
+        if (p.parts == 1) {
+            const bool valid = in && t >= 0.0f && t < (float)(p.n - 1);
+            int next = 0;
+            if (valid) {
+                if constexpr (G == 16) next = after[q * G * K + i];
+                else next = p.next[k * p.n + i];
+            }
+            const float* at = G == 16 ? tile + q * G * K : p.pos + k * p.n;
+            total = end_steps<E, K, G, true>(p, valid, w.map, k, at, i, t, next, mine, total, lane);
+        }
         if (in) (p.parts == 1 ? p.total : p.part_total + (int64_t)w.part * p.maps * p.per * p.n)[k * p.n + i] = total;
     };
 
@@ -497,14 +573,21 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
         const float* pos = p.pos + (w.map * p.per + q0) * (int64_t)p.n;
         if (q0) {
             __syncthreads();
-            stage<K, G>(tile, pos, count, p.n, w.col0, w.cols, w.wave, lane);
+            stage_pass(q0, count);
         }
+        if constexpr (G == 16) __syncthreads();
 #pragma unroll
         for (int x = lane; x < kTile * kWaveRows<G>; x += 64) {
             const int q = x / kWaveRows<G>, r = w.r0 + x % kWaveRows<G>;
-            when_of[x] = q < count && r < p.n ? pos[(int64_t)q * p.n + r] : 65536.0f;
+            float t = 65536.0f;
+            if (q < count && r < p.n) {
+                if constexpr (G == 16) t = tile[q * G * K + r];
+                else t = pos[(int64_t)q * p.n + r];
+            }
+            when_of[x] = t;
         }
-        __syncthreads();
+        if constexpr (G == 16) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        else __syncthreads();
         float z0 = 0.0f, z1 = 0.0f, z2 = 0.0f, z3 = 0.0f;
         for (int a = 0; a < kTile / 4; ++a) {
             z0 = z1; z1 = z2; z2 = z3; z3 = 0.0f;
@@ -688,6 +771,11 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
     }
 }
 
+__device__ __forceinline__ int successor(const LogpParams& p, int64_t k, int r, float when)
+{
+    return p.by_step ? (int)p.tours[k * (p.n + 1) + (int)when + 1] : (int)p.next[k * p.n + r];
+}
+
 // ---- one tour a row: a wave has kSingleRows rows of a tour, 64 / G side by side
 template <int K, int G>
 struct SingleWork {
@@ -790,9 +878,11 @@ __global__ __launch_bounds__(256) void k_single(LogpParams p)
         (p.parts == 1 ? p.top : p.part_top + (int64_t)w.part * p.maps * p.rows)[to] = top;
         (p.parts == 1 ? p.total : p.part_total + (int64_t)w.part * p.maps * p.rows)[to] = total;
     }
-    if (p.parts == 1)
-        end_steps<E, K, G, false>(p, writes && at[0] >= 0.0f && when < (float)(p.n - 1), w.k, w.k, w.r0 + mine, when, top,
-                                  total, lane);
+    if (p.parts == 1) {
+        const bool valid = writes && at[0] >= 0.0f && when < (float)(p.n - 1);
+        end_steps<E, K, G, false>(p, valid, w.k, w.k, at, w.r0 + mine, when,
+                                  valid ? successor(p, w.k, w.r0 + mine, when) : 0, top, total, lane);
+    }
 }
 
 template <typename E, int K, int G>
@@ -873,8 +963,9 @@ __global__ __launch_bounds__(256) void k_join(LogpParams p)
         if (!SHARED || k % p.per == 0) p.top[row] = top;
     }
     const float when = in ? (p.by_step ? (float)r : p.pos[k * p.n + r]) : 0.0f;
-    total = end_steps<E, kMaxPer, 64, SHARED>(p, in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1), map, k, r, when,
-                                              top, total, lane);
+    const bool valid = in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1);
+    total = end_steps<E, kMaxPer, 64, SHARED>(p, valid, map, k, p.pos + k * p.n, r, when,
+                                              valid ? successor(p, k, r, when) : 0, top, total, lane);
     if (in) p.total[w] = total;
 }
 
@@ -1028,13 +1119,15 @@ extern "C" int tsp2opt_tour_logprobs(const void* logits, const int64_t* tours, f
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     LogpParams p = logp_params(logits, tours, state, num_tours, n, tours_per_map, rows, map_stride, row_stride);
     p.logp = logp_out;
-    const size_t lds = 2 * (size_t)n;
-    if (lds > 48 * 1024)
-        HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(k_positions),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    const unsigned threads = n <= 64 ? 64 : n <= 128 ? 128 : n <= 1024 ? 256 : 1024;
-    hipLaunchKernelGGL(k_positions, dim3((unsigned)num_tours), dim3(threads), lds, stream, tours, p.pos, p.next, logp_out,
-                       n);
+    if (tours_per_map == 1 || n > kShortRow) {          // otherwise k_shared makes them itself
+        const size_t lds = 2 * (size_t)n;
+        if (lds > 48 * 1024)
+            HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(k_positions),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        const unsigned threads = n <= 64 ? 64 : n <= 128 ? 128 : n <= 1024 ? 256 : 1024;
+        hipLaunchKernelGGL(k_positions, dim3((unsigned)num_tours), dim3(threads), lds, stream, tours, p.pos, p.next,
+                           logp_out, n);
+    }
     int result = 0;
     T2O_BY_DTYPE(dtype, result = logp_launch<E>(p, false, stream));
     return result;
