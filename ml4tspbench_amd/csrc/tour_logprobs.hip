@@ -277,7 +277,22 @@ __device__ __forceinline__ float scaled_exp(float x)
 
 __device__ __forceinline__ float plain_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// Maximum and sum over a row's open entries by a group of lanes: the steps that k_shared cannot see.
+// The steps that k_shared cannot see, by a group of lanes: h becomes exp(h - top) of the open entries (positions `at`), 0 of
+// the others; top and the sum.
+template <int K, int G>
+__device__ __forceinline__ void open_terms(float (&h)[K], const float (&at)[K], float when, float& top, float& total)
+{
+#pragma unroll
+    for (int x = 0; x < K; ++x) h[x] = at[x] > when ? h[x] : -kInf;
+    top = all<G>(max_of(h), Max());
+    const float from = base_of(top);
+    float s = 0.0f;
+#pragma unroll
+    for (int x = 0; x < K; ++x) s += h[x] = plain_exp(h[x] - from);
+    total = all<G>(s, Add());
+}
+
+// The same for a row of any length, from memory.
 template <typename E, int KK, int G>
 __device__ void open_sum(const E* row, const float* pos, float when, int n, int l, float& top, float& total)
 {
@@ -290,16 +305,13 @@ __device__ void open_sum(const E* row, const float* pos, float when, int n, int 
         Row<float, K> raw_pos;
         load_row<E, K, G>(row + c, l, cols, raw);
         load_row<float, K, G>(pos + c, l, cols, raw_pos);
-        float h[K], at[K], s = 0.0f;
+        float h[K], at[K], m, s;
         end_row<E, K, G>(raw, l, cols, h);
         end_row<float, K, G>(raw_pos, l, cols, at);
-#pragma unroll
-        for (int x = 0; x < K; ++x) h[x] = at[x] > when ? h[x] : -kInf;
-        const float now = vmax(top, all<G>(max_of(h), Max())), from = base_of(now);
-#pragma unroll
-        for (int x = 0; x < K; ++x) s += plain_exp(h[x] - from);
+        open_terms<K, G>(h, at, when, m, s);
+        const float now = vmax(top, m), from = base_of(now);
         if (total != 0.0f) total *= plain_exp(top - from);
-        total += all<G>(s, Add());
+        if (s != 0.0f) total += s * plain_exp(m - from);
         top = now;
     }
 }
@@ -327,16 +339,14 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int src)
     return ((int64_t)__shfl((int)(x >> 32), src) << 32) | (unsigned)__shfl((int)x, src);
 }
 
-// Ends the steps of the lanes with `valid`: (tour k with positions `at`, row r, step `when`, node `next` chosen).  A shared
-// total is 2^60 times the sum; steps of which it says nothing are redone one after the other by their group of lanes:
-// all lanes have to be here.  Returns what the gradient needs to know of the step.
-template <typename E, int K, int G, bool SHARED>
-__device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, const float* at, int r,
-                                           float when, int next, float top, float total, int lane)
+// Ends the steps of the lanes with `valid`: (tour k, row r, step `when`, node `next` chosen).  A shared total is 2^60 times
+// the sum; steps of which it says nothing are redone one after the other by their group of lanes: all lanes have to be
+// here.  redo(lane, top, total) redoes the step of one of a group's lanes (-1: none).  Returns what the gradient needs to know.
+template <typename E, int G, bool SHARED, typename Redo>
+__device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, int r, float when,
+                                           int next, float top, float total, int lane, Redo redo)
 {
-    const E* base = static_cast<const E*>(p.logits);
-    const E* row = base + map * p.map_stride + (int64_t)r * p.row_stride;
-    const int t = (int)when;
+    const E* row = static_cast<const E*>(p.logits) + map * p.map_stride + (int64_t)r * p.row_stride;
     float chosen = 0.0f, keep = total;
     if (valid) chosen = widen(row[next]);
     // log(total) and not of total 2^-60 where that would leave the range of float
@@ -344,15 +354,9 @@ __device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int6
     if (SHARED && total < 0x1p-60f) log_total -= 60.0f / kLog2e;
     if constexpr (SHARED) {
         for (Turns<G> turns(valid && !(total >= kSmall), lane); turns.more();) {
-            const int turn = turns.take(), src = max(turn, 0);
-            const float* pos = reinterpret_cast<const float*>(shfl64(reinterpret_cast<int64_t>(at), src));
-            const int64_t mm = shfl64(map, src);
-            const int rr = __shfl(r, src);
-            const float ww = __shfl(when, src);
+            const int turn = turns.take();
             float m = 0.0f, s = 0.0f;
-            if (turn >= 0)
-                open_sum<E, K, G>(base + mm * p.map_stride + (int64_t)rr * p.row_stride, pos, ww, p.n, lane & (G - 1), m,
-                                  s);
+            redo(turn, m, s);
             if (lane == turn) {
                 top = m;
                 total = s;
@@ -361,7 +365,7 @@ __device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int6
             }
         }
     }
-    if (valid) p.logp[k * (p.n - 1) + t] = total == 0.0f ? -kInf : (chosen - base_of(top)) - log_total;
+    if (valid) p.logp[k * (p.n - 1) + (int)when] = total == 0.0f ? -kInf : (chosen - base_of(top)) - log_total;
     return keep;
 }
 
@@ -562,8 +566,18 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
                 if constexpr (G == 16) next = after[q * G * K + i];
                 else next = p.next[k * p.n + i];
             }
-            const float* at = G == 16 ? tile + q * G * K : p.pos + k * p.n;
-            total = end_steps<E, K, G, true>(p, valid, w.map, k, at, i, t, next, mine, total, lane);
+            total = end_steps<E, G, true>(p, valid, w.map, k, i, t, next, mine, total, lane,
+                                          [&](int turn, float& m, float& s) {
+                const int src = max(turn, 0), qq = __shfl(q, src);      // its positions are in LDS still
+                const float tt = __shfl(t, src);
+                Row<E, K> one;
+                load_row<E, K, G>(row0 + (int64_t)min(w.mine + (src & 3), p.n - 1) * p.row_stride, l, w.cols, one);
+                float h[K], at[K];
+                end_row<E, K, G>(one, l, w.cols, h);
+#pragma unroll
+                for (int x = 0; x < K; ++x) at[x] = tile[qq * G * K + column<K, G>(x, l)];
+                open_terms<K, G>(h, at, tt, m, s);
+            });
         }
         if (in) (p.parts == 1 ? p.total : p.part_total + (int64_t)w.part * p.maps * p.per * p.n)[k * p.n + i] = total;
     };
@@ -642,7 +656,7 @@ __device__ __forceinline__ void join_equal(int& to, float& g)
 template <typename E, int K, int G>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
 {
-    extern __shared__ float tile[];                     // [tours of a pass][G K] positions; in the end [waves][64 K]
+    extern __shared__ float tile[];                     // [tours of a pass][G K] positions, then [waves][64 K]
     __shared__ float4 when[kWaves<G>][kTile][64 / G], weight[kWaves<G>][kTile][64 / G];
     const SharedWork<K, G> w(p);
     const int lane = w.lane, l = w.l;
@@ -712,8 +726,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         join_equal(mine.to, mine.g);
     }
     const bool redo_any = __any(any_redo);
-    __syncthreads();
-    float* const hits = tile + (w.wave * (64 / G) + w.group) * G * K;
+    float* const hits = tile + min(kTile, p.per) * G * K + (w.wave * (64 / G) + w.group) * G * K;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const int i = w.mine + r;
@@ -743,16 +756,28 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
                     const int turn = turns.take(), src = max(turn, 0);
                     const int q = q0 + (once || G == 16 ? src & 15 : src);
                     const float tt = __shfl(own.t, src), gg = __shfl(own.g, src);
-                    if (turn < 0) continue;
+                    float m, total, ex[K], at[K];
                     const float* pos = p.pos + (w.map * p.per + q) * (int64_t)p.n;
-                    float m, total;
-                    open_sum<E, K, G>(row0 - w.col0 + (int64_t)i * p.row_stride, pos, tt, p.n, l, m, total);
-                    const float ws = gg / total;
+                    if (p.per <= kTile) {               // the tile holds all tours still
 #pragma unroll
-                    for (int x = 0; x < K; ++x) {
-                        const int j = column<K, G>(x, l);
-                        if (j < w.cols && pos[w.col0 + j] > tt) d[x] -= ws * plain_exp(h[x] - base_of(m));
+                        for (int x = 0; x < K; ++x) at[x] = tile[q * G * K + column<K, G>(x, l)];
+                    } else {
+                        Row<float, K> raw_pos;
+                        load_row<float, K, G>(pos + w.col0, l, w.cols, raw_pos);
+                        end_row<float, K, G>(raw_pos, l, w.cols, at);
                     }
+                    if (p.parts == 1) {
+#pragma unroll
+                        for (int x = 0; x < K; ++x) ex[x] = h[x];
+                        open_terms<K, G>(ex, at, tt, m, total);
+                    } else {
+                        open_sum<E, K, G>(row0 - w.col0 + (int64_t)i * p.row_stride, pos, tt, p.n, l, m, total);
+#pragma unroll
+                        for (int x = 0; x < K; ++x) ex[x] = at[x] > tt ? plain_exp(h[x] - base_of(m)) : 0.0f;
+                    }
+                    const float ws = turn < 0 ? 0.0f : gg / total;
+#pragma unroll
+                    for (int x = 0; x < K; ++x) d[x] -= at[x] > tt && turn >= 0 ? ws * ex[x] : 0.0f;
                 }
             }
             if (!once) join_equal(s.to, s.g);
@@ -880,8 +905,9 @@ __global__ __launch_bounds__(256) void k_single(LogpParams p)
     }
     if (p.parts == 1) {
         const bool valid = writes && at[0] >= 0.0f && when < (float)(p.n - 1);
-        end_steps<E, K, G, false>(p, valid, w.k, w.k, at, w.r0 + mine, when,
-                                  valid ? successor(p, w.k, w.r0 + mine, when) : 0, top, total, lane);
+        end_steps<E, G, false>(p, valid, w.k, w.k, w.r0 + mine, when,
+                               valid ? successor(p, w.k, w.r0 + mine, when) : 0, top, total, lane,
+                               [](int, float&, float&) {});
     }
 }
 
@@ -964,8 +990,13 @@ __global__ __launch_bounds__(256) void k_join(LogpParams p)
     }
     const float when = in ? (p.by_step ? (float)r : p.pos[k * p.n + r]) : 0.0f;
     const bool valid = in && p.pos[k * p.n] >= 0.0f && when < (float)(p.n - 1);
-    total = end_steps<E, kMaxPer, 64, SHARED>(p, valid, map, k, p.pos + k * p.n, r, when,
-                                              valid ? successor(p, k, r, when) : 0, top, total, lane);
+    total = end_steps<E, 64, SHARED>(p, valid, map, k, r, when, valid ? successor(p, k, r, when) : 0, top, total, lane,
+                                     [&](int turn, float& m, float& s) {
+        const int src = max(turn, 0);
+        const int64_t kk = shfl64(k, src), mm = shfl64(map, src);
+        open_sum<E, kMaxPer, 64>(static_cast<const E*>(p.logits) + mm * p.map_stride + (int64_t)__shfl(r, src) * p.row_stride,
+                                 p.pos + kk * p.n, __shfl(when, src), p.n, lane, m, s);
+    });
     if (in) p.total[w] = total;
 }
 
@@ -1007,7 +1038,7 @@ int logp_rows(LogpParams p, bool grad, hipStream_t stream)
 {
     if (p.per > 1) {
         constexpr int per_block = kWaves<G> * kWaveRows<G>;
-        const int tours = p.per < kTile ? p.per : kTile, words = grad && tours * G < kWaves<G> * 64 ? kWaves<G> * 64 : tours * G;
+        const int words = (p.per < kTile ? p.per : kTile) * G + (grad ? kWaves<G> * 64 : 0);
         p.groups = (p.rows + per_block - 1) / per_block;
         return logp_start(grad ? k_shared_grad<E, K, G> : k_shared<E, K, G>, p, p.maps * p.groups * p.parts,
                           64 * kWaves<G>, sizeof(float) * K * words, stream);
