@@ -13,8 +13,10 @@
 //
 // Several tours a map (k_shared): e_j = exp(h_j - row maximum) does not depend on the tour, only which e_j are added
 // does, and positions are whole numbers, so a masked addition is
-//     S += min(max(pos_j - t, 0), 1) * e_j          (one v_sub with clamp, one v_fmac)
-// instead of an exponential a tour.  That sum loses steps whose open entries all lie far below the row's maximum, so
+//     S += min(max(pos_j - t, 0), 1) * e_j
+// instead of an exponential a tour: a subtraction with clamp and a fused multiply-add.  Up to 2048 nodes, where half
+// floats hold every position exactly, the subtraction takes two entries at a time (v_pk_add_f16 clamp) and
+// v_fma_mix_f32 widens the 0 or 1 on its way into the float sum.  That sum loses steps whose open entries all lie far below the row's maximum, so
 // the exponentials are kept times 2^60, which spends the range of float above 1 too: what it flushes (below 2^-126,
 // 65535 entries at most) is under 2^-30 of a sum above 2^-80, which is 2^-140 = e^-97 relative to the row's maximum.
 // Steps below that (and those that are NaN) are redone alone, relative to their own maximum.
@@ -33,6 +35,7 @@ constexpr int kRows = 4, kTile = 16;                // k_shared: rows of a group
 constexpr int kSingleRows = 16;                     // k_single: rows a wave
 constexpr int kMaxPer = 16;                         // entries of a row a lane holds at most
 constexpr int kShortRow = 256;                      // longest row of a group of 16 lanes
+constexpr int kHalfRow = 2048;                      // up to here half floats hold every position and difference exactly
 
 struct LogpParams {
     const void* logits;
@@ -375,9 +378,73 @@ constexpr int kWaves = G == 64 ? 8 : 4;
 template <int G>
 constexpr int kWaveRows = kRows * 64 / G;               // rows of a wave
 
+using half2 = _Float16 __attribute__((ext_vector_type(2)));
+
+// The steps at which a tour leaves the kRows rows of a group of lanes, as the masks take them.
+template <typename Q>
+struct Leaves {
+    float t[kRows];
+    __device__ __forceinline__ explicit Leaves(const float4& x) : t{x.x, x.y, x.z, x.w} {}
+};
+template <>
+struct Leaves<_Float16> {
+    half2 t[kRows];
+    __device__ __forceinline__ explicit Leaves(const float4& x)
+        : t{__builtin_bit_cast(half2, x.x), __builtin_bit_cast(half2, x.y), __builtin_bit_cast(half2, x.z),
+            __builtin_bit_cast(half2, x.w)} {}
+};
+
+template <typename Q>
+__device__ __forceinline__ float pack_step(float t)
+{
+    if constexpr (sizeof(Q) == 4) return t;
+    const half2 both = {(_Float16)t, (_Float16)t};
+    return __builtin_bit_cast(float, both);
+}
+
+template <typename Q>
+__device__ __forceinline__ float unpack_step(float x)
+{
+    if constexpr (sizeof(Q) == 4) return x;
+    return (float)__builtin_bit_cast(half2, x)[0];
+}
+
+constexpr float kNever = 4096.0f;                       // a step that no position comes after (n <= kHalfRow)
+constexpr float kNeverFloat = 65536.0f;
+
+// f(row, register, mask) for the K entries of a lane and the kRows rows: mask = 1 where the entry's position `at` is behind
+// the step at which the tour leaves the row, else 0.
+template <int K, int G, typename Q, typename F>
+__device__ __forceinline__ void open_masks(const Q* at, int l, const Leaves<Q>& leaves, F f)
+{
+    constexpr int V = kVec<K>;
+    if constexpr (sizeof(Q) == 4 || V == 1) {
+#pragma unroll
+        for (int x = 0; x < K; ++x) {
+            const Q y = at[column<K, G>(x, l)];
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                if constexpr (sizeof(Q) == 4) f(r, x, __builtin_amdgcn_fmed3f(y - leaves.t[r], 0.0f, 1.0f));
+                else f(r, x, (float)__builtin_elementwise_min(__builtin_elementwise_max((_Float16)(y - leaves.t[r][0]), (_Float16)0), (_Float16)1));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < K; x += 2) {
+            const half2 y = *reinterpret_cast<const half2*>(at + column<K, G>(x, l));
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {
+                const half2 m = __builtin_elementwise_min(__builtin_elementwise_max(y - leaves.t[r], (half2)0), (half2)1);
+                f(r, x, (float)m[0]);
+                f(r, x + 1, (float)m[1]);
+            }
+        }
+    }
+}
+
 // The positions of a pass's tours in LDS, a group of 64 lanes a tour; behind the end of a row: -inf, which is never open.
-template <int K, int G>
-__device__ __forceinline__ void stage(float* tile, const float* pos, int count, int n, int col0, int cols, int wave, int lane)
+template <int K, int G, typename Q>
+__device__ __forceinline__ void stage(Q* tile, const float* pos, int count, int n, int col0, int cols, int wave, int lane)
 {
     constexpr int per_wave = kTile / kWaves<G>, C = G * K;
     if constexpr (G == 64) {
@@ -397,7 +464,7 @@ __device__ __forceinline__ void stage(float* tile, const float* pos, int count, 
 #pragma unroll
             for (int c = 0; c < K / V; ++c)
 #pragma unroll
-                for (int v = 0; v < V; ++v) tile[q * C + c * 64 * V + lane * V + v] = at[c * V + v];
+                for (int v = 0; v < V; ++v) tile[q * C + c * 64 * V + lane * V + v] = (Q)at[c * V + v];
         }
     } else {
         constexpr int steps = (C + 63) / 64;
@@ -412,15 +479,15 @@ __device__ __forceinline__ void stage(float* tile, const float* pos, int count, 
 #pragma unroll
             for (int c = 0; c < steps; ++c) {
                 const int q = a * kWaves<G> + wave, j = c * 64 + lane;
-                if (q < count && j < C) tile[q * C + j] = j < cols ? x[a][c] : -kInf;
+                if (q < count && j < C) tile[q * C + j] = (Q)(j < cols ? x[a][c] : -kInf);
             }
     }
 }
 
 // The same from the tours themselves, for rows that fit a workgroup's tile whole (G = 16): k_positions for a pass's
 // tours, a wave a tour, with the successors.  A map's first workgroup also writes them down for the gradient.
-template <int K>
-__device__ __forceinline__ void stage_tours(const LogpParams& p, float* tile, uint16_t* after, int64_t k0, int count,
+template <int K, typename Q>
+__device__ __forceinline__ void stage_tours(const LogpParams& p, Q* tile, uint16_t* after, int64_t k0, int count,
                                             bool writes, int wave, int lane)
 {
     constexpr int C = 16 * K, steps = (C + 63) / 64, per_wave = kTile / kWaves<16>;
@@ -443,14 +510,14 @@ __device__ __forceinline__ void stage_tours(const LogpParams& p, float* tile, ui
             const int s = c * 64 + lane;
             if (s >= p.n) continue;
             if (node[c] < 0) bad = true;
-            else tile[q * C + node[c]] = (float)s;
+            else tile[q * C + node[c]] = (Q)(float)s;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int c = 0; c < steps; ++c) {
             const int s = c * 64 + lane;
             if (s < p.n && node[c] >= 0) {
-                bad |= tile[q * C + node[c]] != (float)s;       // two steps at one node: one of them sees the other's
+                bad |= (float)tile[q * C + node[c]] != (float)s;       // two steps at one node: one of them sees the other's
                 after[q * C + node[c]] = (uint16_t)then[c];
             }
         }
@@ -458,7 +525,7 @@ __device__ __forceinline__ void stage_tours(const LogpParams& p, float* tile, ui
 #pragma unroll
         for (int c = 0; c < steps; ++c) {
             const int j = c * 64 + lane;
-            if (j < C && (bad || j >= p.n)) tile[q * C + j] = j < p.n ? -1.0f : -kInf;
+            if (j < C && (bad || j >= p.n)) tile[q * C + j] = (Q)(j < p.n ? -1.0f : -kInf);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (!writes) continue;
@@ -466,7 +533,7 @@ __device__ __forceinline__ void stage_tours(const LogpParams& p, float* tile, ui
         for (int c = 0; c < steps; ++c) {
             const int j = c * 64 + lane;
             if (j >= p.n) continue;
-            p.pos[k * p.n + j] = tile[q * C + j];
+            p.pos[k * p.n + j] = (float)tile[q * C + j];
             p.next[k * p.n + j] = bad ? (uint16_t)0 : after[q * C + j];
             if (bad && j < p.n - 1) p.logp[k * (p.n - 1) + j] = __builtin_nanf("");
         }
@@ -500,10 +567,11 @@ struct SharedWork {
 // exponential and 8 more an entry of a row.  (Summing over the lanes on the matrix pipe, one v_mfma_f32_16x16x4 a row and
 // tour, takes 10 vector instructions a tour less and 13 us more on 128 maps x 16 tours of 500 nodes: it does not run
 // beside the vector pipe.)
-template <typename E, int K, int G>
+template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 {
-    extern __shared__ float tile[];                     // [tours of a pass][G K] positions
+    extern __shared__ float lds[];
+    Q* const tile = reinterpret_cast<Q*>(lds);          // [tours of a pass][G K] positions
     __shared__ float4 when[kWaves<G>][kTile][64 / G];   // the steps at which the tours leave a wave's rows
     __shared__ uint16_t after[G == 16 ? kTile * 16 * K : 1];
     const SharedWork<K, G> w(p);
@@ -518,9 +586,9 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
         load_row<E, K, G>(row0 + (int64_t)min(w.mine + r, p.n - 1) * p.row_stride, l, w.cols, raw[r]);
     auto stage_pass = [&](int q0, int count) {
         if constexpr (G == 16)
-            stage_tours<K>(p, tile, after, w.map * p.per + q0, count, w.first, w.wave, lane);
+            stage_tours<K, Q>(p, tile, after, w.map * p.per + q0, count, w.first, w.wave, lane);
         else
-            stage<K, G>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
+            stage<K, G, Q>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
     };
     stage_pass(0, min(kTile, p.per));
 #pragma unroll
@@ -556,7 +624,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
     float* const when_of = reinterpret_cast<float*>(when[w.wave]);      // [tour][row of the wave]
     // lane (tour, row i): its step, and its sum where this is the only part
     auto finish = [&](int q0, int q, int count, float total) {
-        const float t = when_of[q * kWaveRows<G> + w.group * kRows + (lane & 3)];
+        const float t = unpack_step<Q>(when_of[q * kWaveRows<G> + w.group * kRows + (lane & 3)]);
         const bool in = q < count && i < p.n;
         const int64_t k = w.map * p.per + q0 + q;
         if (p.parts == 1) {
@@ -575,7 +643,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
                 float h[K], at[K];
                 end_row<E, K, G>(one, l, w.cols, h);
 #pragma unroll
-                for (int x = 0; x < K; ++x) at[x] = tile[qq * G * K + column<K, G>(x, l)];
+                for (int x = 0; x < K; ++x) at[x] = (float)tile[qq * G * K + column<K, G>(x, l)];
                 open_terms<K, G>(h, at, tt, m, s);
             });
         }
@@ -593,12 +661,12 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 #pragma unroll
         for (int x = lane; x < kTile * kWaveRows<G>; x += 64) {
             const int q = x / kWaveRows<G>, r = w.r0 + x % kWaveRows<G>;
-            float t = 65536.0f;
+            float t = sizeof(Q) == 4 ? kNeverFloat : kNever;
             if (q < count && r < p.n) {
-                if constexpr (G == 16) t = tile[q * G * K + r];
+                if constexpr (G == 16) t = (float)tile[q * G * K + r];
                 else t = pos[(int64_t)q * p.n + r];
             }
-            when_of[x] = t;
+            when_of[x] = pack_step<Q>(t);
         }
         if constexpr (G == 16) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         else __syncthreads();
@@ -609,17 +677,10 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
             for (int c = 0; c < 4; ++c) {
                 const int q = 4 * a + c;
                 if (q >= count) continue;
-                const float4 tt = when[w.wave][q][w.group];
-                const float* at = tile + q * G * K;
+                const Leaves<Q> leaves(when[w.wave][q][w.group]);
                 float s[kRows] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int x = 0; x < K; ++x) {
-                    const float y = at[column<K, G>(x, l)];
-                    s[0] = fmaf(__builtin_amdgcn_fmed3f(y - tt.x, 0.0f, 1.0f), e[0][x], s[0]);
-                    s[1] = fmaf(__builtin_amdgcn_fmed3f(y - tt.y, 0.0f, 1.0f), e[1][x], s[1]);
-                    s[2] = fmaf(__builtin_amdgcn_fmed3f(y - tt.z, 0.0f, 1.0f), e[2][x], s[2]);
-                    s[3] = fmaf(__builtin_amdgcn_fmed3f(y - tt.w, 0.0f, 1.0f), e[3][x], s[3]);
-                }
+                open_masks<K, G, Q>(tile + q * G * K, l, leaves,
+                                    [&](int r, int x, float m) { s[r] = fmaf(m, e[r][x], s[r]); });
                 const float sum = quads(s, odd, high, Add());
                 z3 = ((lane >> 2) & 3) == c ? sum : z3;
             }
@@ -653,10 +714,11 @@ __device__ __forceinline__ void join_equal(int& to, float& g)
     if (later) to = -1;
 }
 
-template <typename E, int K, int G>
+template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
 {
-    extern __shared__ float tile[];                     // [tours of a pass][G K] positions, then [waves][64 K]
+    extern __shared__ float lds[];
+    Q* const tile = reinterpret_cast<Q*>(lds);          // [tours of a pass][G K] positions, then [waves][64 K] floats
     __shared__ float4 when[kWaves<G>][kTile][64 / G], weight[kWaves<G>][kTile][64 / G];
     const SharedWork<K, G> w(p);
     const int lane = w.lane, l = w.l;
@@ -667,7 +729,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         int to;
     };
     auto step_of = [&](int q, int i, bool want_to) {
-        Step s{65536.0f, 0.0f, 0.0f, -1};
+        Step s{sizeof(Q) == 4 ? kNeverFloat : kNever, 0.0f, 0.0f, -1};
         if (q >= p.per || i >= p.n) return s;
         const int64_t k = w.map * p.per + q;
         s.t = p.pos[k * p.n + i];
@@ -688,27 +750,22 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
     for (int q0 = 0; q0 < p.per; q0 += kTile) {
         const int count = min(kTile, p.per - q0);
         if (q0) __syncthreads();
-        stage<K, G>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
+        stage<K, G, Q>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
 #pragma unroll
         for (int x = lane; x < kTile * kWaveRows<G>; x += 64) {
             const Step s = step_of(q0 + x / kWaveRows<G>, w.r0 + x % kWaveRows<G>, false);
             const bool redo = unseen(s);
             any_redo |= redo;
-            reinterpret_cast<float*>(when[w.wave])[x] = s.t;
+            reinterpret_cast<float*>(when[w.wave])[x] = pack_step<Q>(s.t);
             reinterpret_cast<float*>(weight[w.wave])[x] = redo || s.g == 0.0f ? 0.0f : s.g / s.total;
         }
         __syncthreads();
         for (int q = 0; q < count; ++q) {
-            const float4 tt = when[w.wave][q][w.group], ww = weight[w.wave][q][w.group];
-            const float* at = tile + q * G * K;
-#pragma unroll
-            for (int x = 0; x < K; ++x) {
-                const float y = at[column<K, G>(x, l)];
-                sum[0][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.x, 0.0f, 1.0f), ww.x, sum[0][x]);
-                sum[1][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.y, 0.0f, 1.0f), ww.y, sum[1][x]);
-                sum[2][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.z, 0.0f, 1.0f), ww.z, sum[2][x]);
-                sum[3][x] = fmaf(__builtin_amdgcn_fmed3f(y - tt.w, 0.0f, 1.0f), ww.w, sum[3][x]);
-            }
+            const Leaves<Q> leaves(when[w.wave][q][w.group]);
+            const float4 ww = weight[w.wave][q][w.group];
+            const float weights[kRows] = {ww.x, ww.y, ww.z, ww.w};
+            open_masks<K, G, Q>(tile + q * G * K, l, leaves,
+                                [&](int r, int x, float m) { sum[r][x] = fmaf(m, weights[r], sum[r][x]); });
         }
     }
     Row<E, K> raw[kRows];
@@ -726,7 +783,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         join_equal(mine.to, mine.g);
     }
     const bool redo_any = __any(any_redo);
-    float* const hits = tile + min(kTile, p.per) * G * K + (w.wave * (64 / G) + w.group) * G * K;
+    float* const hits = reinterpret_cast<float*>(tile + min(kTile, p.per) * G * K) + (w.wave * (64 / G) + w.group) * G * K;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const int i = w.mine + r;
@@ -760,7 +817,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
                     const float* pos = p.pos + (w.map * p.per + q) * (int64_t)p.n;
                     if (p.per <= kTile) {               // the tile holds all tours still
 #pragma unroll
-                        for (int x = 0; x < K; ++x) at[x] = tile[q * G * K + column<K, G>(x, l)];
+                        for (int x = 0; x < K; ++x) at[x] = (float)tile[q * G * K + column<K, G>(x, l)];
                     } else {
                         Row<float, K> raw_pos;
                         load_row<float, K, G>(pos + w.col0, l, w.cols, raw_pos);
@@ -1038,10 +1095,17 @@ int logp_rows(LogpParams p, bool grad, hipStream_t stream)
 {
     if (p.per > 1) {
         constexpr int per_block = kWaves<G> * kWaveRows<G>;
-        const int words = (p.per < kTile ? p.per : kTile) * G + (grad ? kWaves<G> * 64 : 0);
+        const int tours = p.per < kTile ? p.per : kTile;
         p.groups = (p.rows + per_block - 1) / per_block;
-        return logp_start(grad ? k_shared_grad<E, K, G> : k_shared<E, K, G>, p, p.maps * p.groups * p.parts,
-                          64 * kWaves<G>, sizeof(float) * K * words, stream);
+        auto start = [&](auto position) {
+            using Q = decltype(position);
+            return logp_start(grad ? k_shared_grad<E, K, G, Q> : k_shared<E, K, G, Q>, p, p.maps * p.groups * p.parts,
+                              64 * kWaves<G>, (sizeof(Q) * G * tours + (grad ? 256 * kWaves<G> : 0)) * K, stream);
+        };
+        if constexpr (G == 64 && K >= 12) {             // fewer entries a lane only hold shorter rows
+            if (p.n > kHalfRow) return start(float());
+        }
+        return start(_Float16());
     }
     p.groups = (p.rows + kSingleRows - 1) / kSingleRows;
     return logp_start(grad ? k_single_grad<E, K, G> : k_single<E, K, G>, p, (p.maps * p.groups * p.parts + 3) / 4, 256, 0,
