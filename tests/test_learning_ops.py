@@ -293,7 +293,9 @@ gpu = pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
 @pytest.mark.parametrize("M,per,n", [(1, 1, 2), (3, 1, 3), (2, 3, 5), (2, 1, 33), (1, 2, 64), (3, 5, 65), (2, 16, 50),
                                      (1, 17, 100), (2, 4, 129), (1, 40, 37), (1, 3, 333), (2, 1, 257), (1, 2, 512),
-                                     (1, 1, 1025), (1, 3, 1100)])
+                                     (1, 1, 1025), (1, 3, 1100), (1, 2, 13), (1, 18, 16), (2, 3, 17), (1, 33, 96), (2, 2, 190),
+                                     (1, 2, 256), (1, 17, 300), (2, 2, 700), (1, 2, 1024), (1, 2, 2048), (1, 2, 2049),
+                                     (1, 17, 2053), (1, 1, 4097)])
 def test_gpu_log_probs_of_heat_maps(M, per, n, dtype):
     gen = torch.Generator().manual_seed(n * 100 + per)
     check_log_probs(rows_of(gen, M, n, n, dtype), make_tours(gen, M * per, n, start=True), per, "node", gen)
@@ -301,7 +303,8 @@ def test_gpu_log_probs_of_heat_maps(M, per, n, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
-@pytest.mark.parametrize("T,n", [(1, 2), (3, 3), (5, 20), (2, 65), (4, 100), (1, 301), (2, 513), (1, 1026)])
+@pytest.mark.parametrize("T,n", [(1, 2), (3, 3), (5, 20), (2, 65), (4, 100), (1, 301), (2, 513), (1, 1026), (17, 8), (3, 17),
+                                 (2, 193), (1, 255), (2, 257), (1, 769), (1, 2049)])
 def test_gpu_log_probs_of_decoder_rows(T, n, dtype):
     gen = torch.Generator().manual_seed(n)
     check_log_probs(rows_of(gen, T, n - 1, n, dtype), make_tours(gen, T, n), 1, "step", gen)
@@ -311,7 +314,7 @@ def test_gpu_log_probs_of_decoder_rows(T, n, dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
 @pytest.mark.parametrize("per", [1, 2, 7])
 @pytest.mark.parametrize("kind", ["wide", "inf", "lowest"])
-@pytest.mark.parametrize("n", [31, 140, 1030])
+@pytest.mark.parametrize("n", [31, 140, 270, 1030, 2070])
 def test_gpu_log_probs_of_masked_and_wide_rows(n, kind, per, dtype):
     """Rows that run out of entries, entries of the type's lowest value, steps whose open entries all lie far below the
     row's largest: where an exponential relative to the row's largest entry has nothing left."""
@@ -321,7 +324,7 @@ def test_gpu_log_probs_of_masked_and_wide_rows(n, kind, per, dtype):
 
 @gpu
 @pytest.mark.parametrize("per", [1, 3])
-@pytest.mark.parametrize("n", [6, 70, 1031])
+@pytest.mark.parametrize("n", [6, 70, 300, 1031, 2060])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 3.0e38])
 def test_gpu_log_probs_never_use_visited_entries(value, n, per):
     """The diagonal, and every entry that all tours of the map have visited when its row is read, hold poison."""
