@@ -12,6 +12,8 @@
 // little: up to kOneBlock steps one workgroup does everything, sums and end, in one launch.
 #include "learn_common.hpp"
 
+#include <type_traits>
+
 namespace t2o {
 
 constexpr int kMaxBlocks = 2048;        // partial sums the finishing workgroup adds up
@@ -96,6 +98,42 @@ struct Groups {
     }
 };
 
+// f(step) for the steps of a row that thread `at` of a group of G has: four at a time as long as there are, so that
+// their loads are in flight together.  f<N>(first) does steps first, first + G, ..., N of them.
+template <int G, typename F>
+__device__ __forceinline__ void for_steps(int at, int64_t S, F f)
+{
+    int64_t s = at;
+    for (; s + 3 * G < S; s += 4 * G) f(std::integral_constant<int, 4>(), s);
+    for (; s + G < S; s += 2 * G) f(std::integral_constant<int, 2>(), s);
+    if (s < S) f(std::integral_constant<int, 1>(), s);
+}
+
+// The values of steps i, i + G, ...: one branch an array, its loads together.
+template <typename E, int N, int G>
+__device__ __forceinline__ void load_steps(const void* from, int64_t i, bool there, float otherwise, float (&to)[N])
+{
+    if (there) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) to[u] = widen(static_cast<const E*>(from)[i + u * G]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u) to[u] = otherwise;
+    }
+}
+
+template <int N, int G>
+__device__ __forceinline__ void load_kept(const uint8_t* mask, int64_t i, uint8_t (&kept)[N])
+{
+    if (mask) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) kept[u] = mask[i + u * G];
+    } else {
+#pragma unroll
+        for (int u = 0; u < N; ++u) kept[u] = 1;
+    }
+}
+
 __device__ __forceinline__ void policy_end(const PolicyParams& p, const double (&v)[4])
 {
     const double inv = v[3] > 0.0 ? 1.0 / v[3] : 0.0, kl = v[1] * inv;
@@ -112,23 +150,32 @@ __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
     double sum[4] = {0.0, 0.0, 0.0, 0.0};               // ratio term, kl, clipped, weight
     for (int64_t k = g.first; k < p.T; k += g.count) {
         double v[5] = {0.0, 0.0, 0.0, 0.0, 0.0};        // ratio term, kl, clipped, steps, difference of the tour
-        for (int64_t s = g.at; s < p.S; s += G) {
-            const int64_t i = k * p.S + s;
-            const float lp = widen(static_cast<const E*>(p.lp)[i]), old = widen(static_cast<const E*>(p.old)[i]);
-            const float ref = p.ref ? widen(static_cast<const E*>(p.ref)[i]) : lp;
-            if (p.mask && !p.mask[i]) continue;
-            const double x = (double)lp - (double)old;
-            v[3] += 1.0;
-            if (p.mode & kRatioTour) {
-                v[4] += x;
-            } else {
-                const float adv = p.adv[p.adv_per_step ? i : k];
-                const bool cut = is_cut(p, adv, x);
-                v[0] += (double)(-adv * (cut ? (adv > 0.0f ? p.hi : p.lo) : expf((float)x)));
-                v[2] += cut ? 1.0 : 0.0;
+        const float of_tour = p.adv_per_step ? 0.0f : p.adv[k];
+        for_steps<G>(g.at, p.S, [&](auto many, int64_t first) {
+            constexpr int N = decltype(many)::value;
+            float lp[N], old[N], ref[N], adv[N];
+            uint8_t kept[N];
+            const int64_t i = k * p.S + first;
+            load_steps<E, N, G>(p.lp, i, true, 0.0f, lp);
+            load_steps<E, N, G>(p.old, i, true, 0.0f, old);
+            load_steps<E, N, G>(p.ref, i, p.ref, 0.0f, ref);
+            load_steps<float, N, G>(p.adv, i, p.adv_per_step, of_tour, adv);
+            load_kept<N, G>(p.mask, i, kept);
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                if (!kept[u]) continue;
+                const double x = (double)lp[u] - (double)old[u];
+                v[3] += 1.0;
+                if (p.mode & kRatioTour) {
+                    v[4] += x;
+                } else {
+                    const bool cut = is_cut(p, adv[u], x);
+                    v[0] += (double)(-adv[u] * (cut ? (adv[u] > 0.0f ? p.hi : p.lo) : expf((float)x)));
+                    v[2] += cut ? 1.0 : 0.0;
+                }
+                if (p.ref) v[1] += (double)kl_term(ref[u] - lp[u]);
             }
-            if (p.ref) v[1] += (double)kl_term(ref - lp);
-        }
+        });
         if (p.mode == 0) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) sum[c] += v[c];
@@ -176,26 +223,36 @@ __global__ __launch_bounds__(1024) void k_policy_grad(PolicyParams p)
     const float scale = (float)(p.norm[0] * (double)p.g[0]);
     for (int64_t k = g.first; k < p.T; k += g.count) {
         const float2 row = p.mode ? p.rows[k] : make_float2(0.0f, 1.0f);
-        for (int64_t s = g.at; s < p.S; s += G) {
-            const int64_t i = k * p.S + s;
-            float d = 0.0f;
-            if (!p.mask || p.mask[i]) {
-                const float lp = widen(static_cast<const E*>(p.lp)[i]);
-                if (p.mode & kRatioTour) {
-                    d = row.x;
-                } else {
-                    const double x = (double)lp - (double)widen(static_cast<const E*>(p.old)[i]);
-                    const float adv = p.adv[p.adv_per_step ? i : k];
-                    d = is_cut(p, adv, x) ? 0.0f : -adv * expf((float)x) * row.y;
+        const float of_tour = p.adv_per_step ? 0.0f : p.adv[k];
+        for_steps<G>(g.at, p.S, [&](auto many, int64_t first) {
+            constexpr int N = decltype(many)::value;
+            float lp[N], old[N], ref[N], adv[N];
+            uint8_t kept[N];
+            const int64_t i = k * p.S + first;
+            load_steps<E, N, G>(p.lp, i, true, 0.0f, lp);
+            load_steps<E, N, G>(p.old, i, !(p.mode & kRatioTour), 0.0f, old);
+            load_steps<E, N, G>(p.ref, i, p.ref && p.kl_coef != 0.0, 0.0f, ref);
+            load_steps<float, N, G>(p.adv, i, p.adv_per_step, of_tour, adv);
+            load_kept<N, G>(p.mask, i, kept);
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                float d = 0.0f;
+                if (kept[u]) {
+                    if (p.mode & kRatioTour) {
+                        d = row.x;
+                    } else {
+                        const double x = (double)lp[u] - (double)old[u];
+                        d = is_cut(p, adv[u], x) ? 0.0f : -adv[u] * expf((float)x) * row.y;
+                    }
+                    if (p.ref && p.kl_coef != 0.0) {
+                        const float e = ref[u] - lp[u];
+                        d -= (float)p.kl_coef * row.y * (fabsf(e) > 1.0f ? expf(e) - 1.0f : kl_term(e) + e);
+                    }
+                    d *= scale;
                 }
-                if (p.ref && p.kl_coef != 0.0) {
-                    const float e = widen(static_cast<const E*>(p.ref)[i]) - lp;
-                    d -= (float)p.kl_coef * row.y * (fabsf(e) > 1.0f ? expf(e) - 1.0f : kl_term(e) + e);
-                }
-                d *= scale;
+                static_cast<E*>(p.grad)[i + u * G] = narrow<E>(d);
             }
-            static_cast<E*>(p.grad)[i] = narrow<E>(d);
-        }
+        });
     }
 }
 
@@ -224,14 +281,20 @@ __device__ __forceinline__ void pref_rows(const PrefParams& p)
     const Groups<G> g;
     for (int64_t k = g.first; k < p.T; k += g.count) {
         double v[2] = {0.0, 0.0};                       // sum, steps
-        for (int64_t s = g.at; s < p.S; s += G) {
-            const int64_t i = k * p.S + s;
-            const double lp = (double)widen(static_cast<const E*>(p.lp)[i]);
-            const double ref = p.ref ? (double)widen(static_cast<const E*>(p.ref)[i]) : 0.0;
-            if (p.mask && !p.mask[i]) continue;
-            v[0] += lp - ref;
-            v[1] += 1.0;
-        }
+        for_steps<G>(g.at, p.S, [&](auto many, int64_t first) {
+            constexpr int N = decltype(many)::value;
+            float lp[N], ref[N];
+            uint8_t kept[N];
+            const int64_t i = k * p.S + first;
+            load_steps<E, N, G>(p.lp, i, true, 0.0f, lp);
+            load_steps<E, N, G>(p.ref, i, p.ref, 0.0f, ref);
+            load_kept<N, G>(p.mask, i, kept);
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                v[0] += kept[u] ? (double)lp[u] - (double)ref[u] : 0.0;
+                v[1] += kept[u] ? 1.0 : 0.0;
+            }
+        });
         group_sum<G>(v);
         if (g.at == 0) {
             const double scale = p.per_step ? p.beta / fmax(v[1], 1.0) : p.beta;
@@ -361,7 +424,7 @@ struct Shape {
 Shape shape_of(int64_t T, int64_t S, bool one_block)
 {
     Shape s;
-    s.group = S <= 24 ? 8 : S > 2048 && T < 2048 ? kBlockRow : 64;
+    s.group = S <= 24 ? 8 : S <= 160 ? 16 : S > 2048 && T < 2048 ? kBlockRow : 64;
     s.threads = s.group == kBlockRow || one_block ? 1024 : 256;
     const int64_t grid = (T * s.group + s.threads - 1) / s.threads;
     s.grid = one_block ? 1u : (unsigned)(grid < kMaxBlocks ? grid : kMaxBlocks);
@@ -371,6 +434,7 @@ Shape shape_of(int64_t T, int64_t S, bool one_block)
 #define T2O_BY_GROUP(group, CALL)                                  \
     switch (group) {                                               \
         case 8: { constexpr int G = 8; CALL; break; }              \
+        case 16: { constexpr int G = 16; CALL; break; }            \
         case 64: { constexpr int G = 64; CALL; break; }            \
         default: { constexpr int G = kBlockRow; CALL; break; }     \
     }
