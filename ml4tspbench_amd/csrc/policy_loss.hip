@@ -7,9 +7,10 @@
 // Both are averages; the gradients are recomputed from the same inputs in one pass.  Sums over steps and rows are
 // kept in double and added in a fixed order: results do not depend on the schedule.
 //
-// A row of steps is read by a group of G threads: 8 for short rows (eight rows a wave), a wave, or for long rows of few
-// tours a whole workgroup.  Bound by memory where there is much, by the launches and the host's autograd where there is
-// little: up to kOneBlock steps one workgroup does everything, sums and end, in one launch.
+// A row of steps is read by a group of G threads: 8 or 16 for short rows, a wave, or for long rows of few tours a whole
+// workgroup.  Bound by memory where there is much (10000 x 1000 steps in float32 with reference and mask: 130 MB read in
+// 39 us, 3.4 TB/s, and 170 MB moved by the gradient in 33 us, 5.2 TB/s), by the launches and the host's autograd where
+// there is little: up to kOneBlock steps one workgroup does everything, sums and end, in one launch.
 #include "learn_common.hpp"
 
 #include <type_traits>
@@ -18,7 +19,7 @@ namespace t2o {
 
 constexpr int kMaxBlocks = 2048;        // partial sums the finishing workgroup adds up
 constexpr int kBlockRow = 1024;         // threads of a workgroup that has a row to itself
-constexpr int64_t kOneBlock = 16384;    // steps that one workgroup of kOneThreads takes in one launch
+constexpr int64_t kOneBlock = 8192;     // steps that one workgroup of kOneThreads takes in one launch
 constexpr int kOneThreads = 1024;
 constexpr int kRatioTour = 1, kAverageTour = 2;
 
@@ -415,7 +416,15 @@ int loss_check(int64_t T, int64_t S, int32_t dtype)
 
 bool off(const void* ptr, size_t size) { return reinterpret_cast<uintptr_t>(ptr) % size != 0; }
 
-// How rows of S steps are shared out: threads a row, threads a workgroup, workgroups.
+// How rows of S steps are shared out: threads a row, threads a workgroup, workgroups.  Values and gradient in us, float32
+// with reference and mask:            8 threads     16            64            1024
+//   100000 tours x 10 steps           17.5 +  9     22.5 +  9     76.5 +  31
+//    50000 x 24                       14   + 7.5    18   +  9     45   +  17
+//    20000 x 150                      18   + 14     17.5 + 12     28   + 15.5
+//    10000 x 499                      35   + 31     25   + 21     27   + 19
+//     1500 x 3000 (ratio of tours)   129   + 94     68   + 49     23   + 17     74   + 16
+//       16 x 10000 (ratio of tours)  414   + 245   208   + 120    42   + 32     16.5 + 6.5
+// One workgroup alone, 160 x 100: 15 us in one launch against 6.6 + 5.3 us in two and 3.5 us more on the host.
 struct Shape {
     int group, threads;
     unsigned grid;
@@ -424,7 +433,7 @@ struct Shape {
 Shape shape_of(int64_t T, int64_t S, bool one_block)
 {
     Shape s;
-    s.group = S <= 24 ? 8 : S <= 160 ? 16 : S > 2048 && T < 2048 ? kBlockRow : 64;
+    s.group = S <= 24 ? 8 : S <= 160 ? 16 : S > 2048 && T <= 256 ? kBlockRow : 64;
     s.threads = s.group == kBlockRow || one_block ? 1024 : 256;
     const int64_t grid = (T * s.group + s.threads - 1) / s.threads;
     s.grid = one_block ? 1u : (unsigned)(grid < kMaxBlocks ? grid : kMaxBlocks);
