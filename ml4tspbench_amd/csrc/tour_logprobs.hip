@@ -1035,13 +1035,15 @@ __global__ __launch_bounds__(256) void k_single_grad(LogpParams p)
     }
 }
 
-// Puts the parts of long rows together and ends their steps: one lane a (tour, row).
+// Puts the parts of long rows together and ends their steps: one lane a (tour, row).  Where steps may have to be redone,
+// one after the other in a wave, a wave has 16 of them: 7 maps x 3 tours of 1704 nodes with 10 neighbours 40 -> 23 us.
 template <typename E, bool SHARED>
 __global__ __launch_bounds__(256) void k_join(LogpParams p)
 {
+    constexpr int per_wave = SHARED ? 16 : 64;
     const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x, every = p.maps * p.per * p.rows;
-    const bool in = w < every;
+    const int64_t w = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * per_wave + lane, every = p.maps * p.per * p.rows;
+    const bool in = lane < per_wave && w < every;
     const int64_t k = in ? w / p.rows : 0, map = SHARED ? k / p.per : k;
     const int r = in ? (int)(w - k * p.rows) : 0;
     const int64_t row = map * p.rows + r;
@@ -1135,7 +1137,7 @@ int logp_launch(LogpParams p, bool grad, hipStream_t stream)
     else T2O_BY_HELD(k, (rc = logp_rows<E, K < 6 ? 6 : K, 64>(p, grad, stream)))
     if (rc) return rc;
     if (!grad && p.parts > 1) {
-        const int64_t blocks = (p.maps * p.per * p.rows + 255) / 256;
+        const int64_t items = p.per > 1 ? 64 : 256, blocks = (p.maps * p.per * p.rows + items - 1) / items;
         rc = logp_start(p.per > 1 ? k_join<E, true> : k_join<E, false>, p, blocks, 256, 0, stream);
         if (rc) return rc;
     }
