@@ -274,6 +274,7 @@ int tsp2opt_gls_rounds(const double* points, int64_t* tours, int64_t* best_tours
  * Entries of visited nodes (the diagonal among them) are never used, whatever they hold.  A step whose open entries
  * are all -inf gets -inf, a chosen -inf among finite ones too; NaN or +inf among the open entries gives NaN.  A tour
  * that is no permutation of 0 .. n-1 gets NaN in all its steps and adds nothing to the gradient.
+ * Batches whose launches would have 2^32 threads (10^9 choices and more) give TSP2OPT_E_UNSUPPORTED.
  * tsp2opt_tour_logprobs_grad -- grad_out (same shape as logits, contiguous, same dtype) from grad_logp
  * (num_tours, n-1) float.  A step whose grad_logp is 0, or whose open entries are all -inf, adds nothing.
  */

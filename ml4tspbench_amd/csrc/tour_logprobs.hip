@@ -1094,51 +1094,73 @@ inline int held(int n)
         default: { constexpr int K = 16; CALL; break; }     \
     }
 
+// Launch shape of the kernels of one call, and whether a launch takes it: a grid of 2^32 threads or more starts nothing.
+struct LogpShape {
+    int k, parts, tours, position_threads;
+    int64_t groups, rows_grid, rows_threads, join_grid;
+    bool fits;
+    LogpShape(int64_t T, int n, int rows, int per)
+    {
+        k = held(n);
+        parts = parts_of(n);
+        tours = per < kTile ? per : kTile;
+        position_threads = n <= 64 ? 64 : n <= 128 ? 128 : n <= 1024 ? 256 : 1024;
+        const int64_t maps = T / per;
+        if (per > 1) {
+            const int block = n <= kShortRow ? kWaves<16> * kWaveRows<16> : kWaves<64> * kWaveRows<64>;
+            rows_threads = 64 * (n <= kShortRow ? kWaves<16> : kWaves<64>);
+            groups = (rows + block - 1) / block;
+            rows_grid = maps * groups * parts;
+        } else {
+            rows_threads = 256;
+            groups = (rows + kSingleRows - 1) / kSingleRows;
+            rows_grid = (maps * groups * parts + 3) / 4;
+        }
+        const int64_t items = per > 1 ? 64 : 256;
+        join_grid = parts > 1 ? (T * rows + items - 1) / items : 0;
+        fits = T * position_threads < (int64_t)1 << 32 && rows_grid * rows_threads < (int64_t)1 << 32 &&
+               join_grid * 256 < (int64_t)1 << 32;
+    }
+};
+
 template <typename Kernel>
-int logp_start(Kernel kern, LogpParams p, int64_t grid, int threads, size_t lds, hipStream_t stream)
+int logp_start(Kernel kern, const LogpParams& p, int64_t grid, int64_t threads, size_t lds, hipStream_t stream)
 {
-    if (grid > 0x7fffffffll) return fail(TSP2OPT_E_UNSUPPORTED, "too many rows");
     if (lds > 48 * 1024)
         HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize,
                                     (int)lds));
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(threads), lds, stream, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3((unsigned)threads), lds, stream, p);
     return 0;
 }
 
 template <typename E, int K, int G>
-int logp_rows(LogpParams p, bool grad, hipStream_t stream)
+int logp_rows(const LogpParams& p, const LogpShape& s, bool grad, hipStream_t stream)
 {
     if (p.per > 1) {
-        constexpr int per_block = kWaves<G> * kWaveRows<G>;
-        const int tours = p.per < kTile ? p.per : kTile;
-        p.groups = (p.rows + per_block - 1) / per_block;
         auto start = [&](auto position) {
             using Q = decltype(position);
-            return logp_start(grad ? k_shared_grad<E, K, G, Q> : k_shared<E, K, G, Q>, p, p.maps * p.groups * p.parts,
-                              64 * kWaves<G>, (sizeof(Q) * G * tours + (grad ? 256 * kWaves<G> : 0)) * K, stream);
+            return logp_start(grad ? k_shared_grad<E, K, G, Q> : k_shared<E, K, G, Q>, p, s.rows_grid, s.rows_threads,
+                              (sizeof(Q) * G * s.tours + (grad ? 256 * kWaves<G> : 0)) * K, stream);
         };
         if constexpr (G == 64 && K >= 12) {             // fewer entries a lane only hold shorter rows
             if (p.n > kHalfRow) return start(float());
         }
         return start(_Float16());
     }
-    p.groups = (p.rows + kSingleRows - 1) / kSingleRows;
-    return logp_start(grad ? k_single_grad<E, K, G> : k_single<E, K, G>, p, (p.maps * p.groups * p.parts + 3) / 4, 256, 0,
-                      stream);
+    return logp_start(grad ? k_single_grad<E, K, G> : k_single<E, K, G>, p, s.rows_grid, s.rows_threads, 0, stream);
 }
 
 template <typename E>
-int logp_launch(LogpParams p, bool grad, hipStream_t stream)
+int logp_launch(LogpParams p, const LogpShape& s, bool grad, hipStream_t stream)
 {
-    p.parts = parts_of(p.n);
-    const int k = held(p.n);
+    p.parts = s.parts;
+    p.groups = s.groups;
     int rc = 0;
-    if (p.n <= kShortRow) T2O_BY_HELD(k, (rc = logp_rows<E, K, 16>(p, grad, stream)))
-    else T2O_BY_HELD(k, (rc = logp_rows<E, K < 6 ? 6 : K, 64>(p, grad, stream)))
+    if (p.n <= kShortRow) T2O_BY_HELD(s.k, (rc = logp_rows<E, K, 16>(p, s, grad, stream)))
+    else T2O_BY_HELD(s.k, (rc = logp_rows<E, K < 6 ? 6 : K, 64>(p, s, grad, stream)))
     if (rc) return rc;
     if (!grad && p.parts > 1) {
-        const int64_t items = p.per > 1 ? 64 : 256, blocks = (p.maps * p.per * p.rows + items - 1) / items;
-        rc = logp_start(p.per > 1 ? k_join<E, true> : k_join<E, false>, p, blocks, 256, 0, stream);
+        rc = logp_start(p.per > 1 ? k_join<E, true> : k_join<E, false>, p, s.join_grid, 256, 0, stream);
         if (rc) return rc;
     }
     HIP_TRY(hipGetLastError());
@@ -1156,7 +1178,7 @@ int logp_check(const void* logits, const int64_t* tours, const void* out, const 
     const int size = element_size(dtype);
     if (!size) return fail(TSP2OPT_E_ARG, "dtype must be float32, bfloat16 or float16");
     if (map_stride < 0 || row_stride < 0) return fail(TSP2OPT_E_ARG, "negative stride");
-    if (num_tours > 0x7fffffffll || num_tours * (int64_t)n > (int64_t)1 << 32)
+    if (num_tours > 0x7fffffffll || !LogpShape(num_tours, n, by_step ? n - 1 : n, per).fits)
         return fail(TSP2OPT_E_UNSUPPORTED, "too many tours");
     if (num_tours == 0 || n == 1) return 0;
     if (!logits || !tours || !out || !state) return fail(TSP2OPT_E_ARG, "null pointer");
@@ -1229,17 +1251,17 @@ extern "C" int tsp2opt_tour_logprobs(const void* logits, const int64_t* tours, f
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     LogpParams p = logp_params(logits, tours, state, num_tours, n, tours_per_map, rows, map_stride, row_stride);
     p.logp = logp_out;
+    const LogpShape shape(num_tours, n, p.rows, tours_per_map);
     if (tours_per_map == 1 || n > kShortRow) {          // otherwise k_shared makes them itself
         const size_t lds = 2 * (size_t)n;
         if (lds > 48 * 1024)
             HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(k_positions),
                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        const unsigned threads = n <= 64 ? 64 : n <= 128 ? 128 : n <= 1024 ? 256 : 1024;
-        hipLaunchKernelGGL(k_positions, dim3((unsigned)num_tours), dim3(threads), lds, stream, tours, p.pos, p.next,
-                           logp_out, n);
+        hipLaunchKernelGGL(k_positions, dim3((unsigned)num_tours), dim3(shape.position_threads), lds, stream, tours, p.pos,
+                           p.next, logp_out, n);
     }
     int result = 0;
-    T2O_BY_DTYPE(dtype, result = logp_launch<E>(p, false, stream));
+    T2O_BY_DTYPE(dtype, result = logp_launch<E>(p, shape, false, stream));
     return result;
 }
 
@@ -1265,6 +1287,6 @@ extern "C" int tsp2opt_tour_logprobs_grad(const void* logits, const int64_t* tou
     p.g = grad_logp;
     p.grad = grad_out;
     int result = 0;
-    T2O_BY_DTYPE(dtype, result = logp_launch<E>(p, true, stream));
+    T2O_BY_DTYPE(dtype, result = logp_launch<E>(p, LogpShape(num_tours, n, p.rows, tours_per_map), true, stream));
     return result;
 }

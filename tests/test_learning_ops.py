@@ -234,6 +234,7 @@ def test_c_abi_checks_without_gpu():
     assert L.tsp2opt_tour_logprobs_state_bytes(5, 10, 2, 0) == -1 and L.tsp2opt_tour_logprobs_state_bytes(4, 0, 2, 0) == -1
     assert logp(n=0) == -1 and logp(T=-2) == -1 and logp(T=3) == -1 and logp(per=0) == -1
     assert logp(n=70000) == -2 and logp(T=1 << 31, per=1) == -2
+    assert logp(T=1 << 26, per=1) == -2 and logp(T=1 << 25, n=200, per=2) == -2      # launches of 2^32 threads
     assert logp(rows=2) == -1 and logp(rows=1) == -1 and logp(dt=1) == -1 and logp(ms=-1) == -1
     assert logp(logits=None) == -1 and logp(state=None) == -1
     assert logp(logits=at2) == -1 and b"misaligned" in L.tsp2opt_last_error()
@@ -685,6 +686,42 @@ def test_gpu_captured_step_replays_like_the_eager_one():
         torch.cuda.synchronize()
         for o, w in zip(outs, want):
             assert all(torch.equal(p, q) for p, q in zip(o, w))
+
+
+@gpu
+def test_gpu_without_gradients():
+    """no_grad, inference mode and inputs that need none: the same values, nothing kept."""
+    import ml4tspbench_amd as amd
+    heat, tours, old, adv, length, per = step_inputs(6)
+    want = amd.tour_log_probs(heat.clone().requires_grad_(), tours, tours_per_map=per)
+    pol, pref = amd.clipped_policy_loss(want, old, adv), amd.preference_loss(want, length, tours_per_instance=per)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            got = amd.tour_log_probs(heat.clone(), tours.clone(), tours_per_map=per)
+            a = amd.clipped_policy_loss(got, old.clone(), adv.clone(), mask=torch.ones_like(got, dtype=torch.bool))
+            b = amd.preference_loss(got, length.clone(), tours_per_instance=per)
+        assert not got.requires_grad and torch.equal(got, want.detach())
+        assert torch.equal(a.loss, pol.loss.detach()) and torch.equal(b.loss, pref.loss.detach())
+    assert not amd.tour_log_probs(heat, tours, tours_per_map=per).requires_grad
+
+
+@gpu
+def test_gpu_broadcast_maps_and_graph_kept_for_two_backwards():
+    """One heat map expanded over several entries of the batch: its gradient is their sum; a graph used twice."""
+    import ml4tspbench_amd as amd
+    gen = torch.Generator().manual_seed(14)
+    n, M, per = 55, 3, 2
+    tours = make_tours(gen, M * per, n).cuda()
+    one = rows_of(gen, 1, n, n, torch.float32).cuda()
+    a, b = one.clone().requires_grad_(), one.expand(M, n, n).contiguous().requires_grad_()
+    g = torch.randn((M * per, n - 1), generator=gen).cuda()
+    lp = amd.tour_log_probs(a.expand(M, n, n), tours, tours_per_map=per)
+    first = torch.autograd.grad(lp, a, g, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(lp, a, g)[0])
+    want = amd.tour_log_probs(b, tours, tours_per_map=per)
+    assert torch.equal(lp.detach(), want.detach())
+    (each,) = torch.autograd.grad(want, b, g)
+    assert torch.allclose(first, each.sum(0, keepdim=True), rtol=4 * U * M, atol=4 * U * M * float(each.abs().max()))
 
 
 @gpu
