@@ -721,16 +721,19 @@ __device__ __forceinline__ void join_equal(int& to, float& g)
 }
 
 // sum_q g_q / S_q [open in tour q] for every entry of a row by the same masked additions, times its exponential, plus g at
-// the chosen entries.  128 maps x 16 tours of 500 nodes in bfloat16: 73 us for 128 MB (27 us at the rate of a large copy);
-// bound by its vector instructions, of which half are the masked additions.
+// the chosen entries.  128 maps x 16 tours of 500 nodes in bfloat16: 69 us for 128 MB (27 us at the rate of a large copy), of which
+// 20 are the masked additions and 7 the choices (copies without them take so much less);
+// the rest is reading positions, steps and rows one after the other.
 template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
 {
     extern __shared__ float lds[];
     Q* const tile = reinterpret_cast<Q*>(lds);          // [tours of a pass][G K] positions, then [waves][64 K] floats
     __shared__ float4 when[kWaves<G>][kTile][64 / G], weight[kWaves<G>][kTile][64 / G];
+    __shared__ float2 choice[G == 64 ? kWaves<G> : 1][kTile * kRows];     // of the steps: gradient; entry, bit 20: to be redone
     const SharedWork<K, G> w(p);
     const int lane = w.lane, l = w.l;
+    const bool once = G == 64 && p.per <= kTile;        // 16 lanes a row: the four rows' choices at one go
     const E* row0 = static_cast<const E*>(p.logits) + w.map * p.map_stride + w.col0;
     // what the gradient of tour q's step that leaves row i takes; g = 0: nothing
     struct Step {
@@ -745,7 +748,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         if (!(s.t >= 0.0f && s.t < (float)(p.n - 1))) return s;
         s.total = p.total[k * p.n + i];
         if (s.total != kDead) s.g = p.g[k * (p.n - 1) + (int)s.t];
-        if (want_to && s.g != 0.0f) s.to = (int)p.next[k * p.n + i] - w.col0;
+        if (want_to && s.g != 0.0f) s.to = (int)p.next[k * p.n + i];
         return s;
     };
     auto unseen = [](const Step& s) { return s.g != 0.0f && (!(s.total >= kSmall) || !(fabsf(s.g / s.total) < kInf)); };
@@ -762,9 +765,10 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         stage<K, G, Q>(tile, p.pos + (w.map * p.per + q0) * (int64_t)p.n, count, p.n, w.col0, w.cols, w.wave, lane);
 #pragma unroll
         for (int x = lane; x < kTile * kWaveRows<G>; x += 64) {
-            const Step s = step_of(q0 + x / kWaveRows<G>, w.r0 + x % kWaveRows<G>, false);
+            const Step s = step_of(q0 + x / kWaveRows<G>, w.r0 + x % kWaveRows<G>, once);
             const bool redo = unseen(s);
             any_redo |= redo;
+            if (once) choice[w.wave][x] = make_float2(s.g, __int_as_float(redo ? s.to | 1 << 20 : s.to));
             reinterpret_cast<float*>(when[w.wave])[x] = pack_step<Q>(s.t);
             reinterpret_cast<float*>(weight[w.wave])[x] = redo || s.g == 0.0f ? 0.0f : s.g / s.total;
         }
@@ -783,12 +787,17 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         load_row<E, K, G>(row0 + (int64_t)min(w.mine + r, p.n - 1) * p.row_stride, l, w.cols, raw[r]);
     // + g at the chosen entries, through LDS: a row of zeros, the choices of 16 tours added with equal ones joined first
     // (all lanes then write different entries), further tours after them in their order.
-    const bool once = G == 64 && p.per <= 16;           // 16 lanes a row: the four rows' choices at one go
     Step mine{};
+    float g_mine = 0.0f;
     bool redo_mine = false;
     if (once) {
-        mine = step_of(lane & 15, w.mine + (lane >> 4), true);
-        redo_mine = unseen(mine);
+        const int x = (lane & 15) * kRows + (lane >> 4);
+        const float2 c = choice[w.wave][x];
+        mine.t = unpack_step<Q>(reinterpret_cast<const float*>(when[w.wave])[x]);
+        g_mine = mine.g = c.x;
+        mine.to = __float_as_int(c.y);
+        redo_mine = mine.to >= 0 && (mine.to & 1 << 20);
+        if (mine.to >= 0) mine.to &= (1 << 20) - 1;
         join_equal(mine.to, mine.g);
     }
     const bool redo_any = __any(any_redo);
@@ -817,11 +826,11 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
             }
             if (redo_any) {
                 const bool todo = once ? redo_mine && (lane >> 4) == r : unseen(s);
-                const Step own = once ? step_of(lane & 15, w.mine + (lane >> 4), false) : s;
+                const float t_own = once ? mine.t : s.t, g_own = once ? g_mine : s.g;
                 for (Turns<G> turns(todo, lane); turns.more();) {
                     const int turn = turns.take(), src = max(turn, 0);
                     const int q = q0 + (once || G == 16 ? src & 15 : src);
-                    const float tt = __shfl(own.t, src), gg = __shfl(own.g, src);
+                    const float tt = __shfl(t_own, src), gg = __shfl(g_own, src);
                     float m, total, ex[K], at[K];
                     const float* pos = p.pos + (w.map * p.per + q) * (int64_t)p.n;
                     if (p.per <= kTile) {               // the tile holds all tours still
@@ -847,11 +856,12 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
                 }
             }
             if (!once) join_equal(s.to, s.g);
-            const bool hit = s.to >= 0 && s.to < w.cols;
+            const int at = s.to - w.col0;
+            const bool hit = at >= 0 && at < w.cols;
 #pragma unroll
             for (int c = 0; c < (G == 64 ? 4 : 1); ++c)
                 if (hit && (G == 16 || (lane >> 4) == c))
-                    __hip_atomic_fetch_add(&hits[s.to], s.g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                    __hip_atomic_fetch_add(&hits[at], s.g, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
