@@ -52,6 +52,9 @@ def main():
     ap.add_argument("--max-iterations", type=int, default=5000)
     ap.add_argument("--cluster-mode", type=int, default=-1, help="diagnostic, see bench.py")
     ap.add_argument("--phases", action="store_true", help="diagnostic: phase cycles of one extra 2-opt run")
+    ap.add_argument("--learn", action="store_true",
+                    help="also time a training step on the heat maps: the decoded and the improved tours scored, a "
+                         "preference and a policy loss, and the gradient")
     ap.add_argument("--tune", action="append", default=[], help="diagnostic: tsp2opt_debug_tune what=value")
     args = ap.parse_args()
     if not torch.cuda.is_available():
@@ -135,6 +138,32 @@ def main():
                          "dense_decode_ms": float(ev[0].elapsed_time(ev[1])),
                          "dense_key_bytes": int(inst * per * n * n * 8),
                          "same_tours_as_dense_decode": bool(torch.equal(dense_tours, tours))}
+    if args.learn:
+        # the improved tours preferred over the decoded ones, and reinforced by how much shorter they are
+        logits = heat.clamp(min=torch.finfo(heat.dtype).tiny).log_().requires_grad_()
+        both = torch.stack([tours, res.tours], 1).view(-1, n + 1)
+        length = amd.evaluate_tours(pts, both, tours_per_instance=2 * per).lengths
+        adv = (length.view(inst, -1).mean(1, keepdim=True) - length.view(inst, -1)).flatten()
+
+        def learn():
+            ev = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
+            ev[0].record()
+            lp = amd.tour_log_probs(logits, both, tours_per_map=2)
+            ev[1].record()
+            loss = amd.preference_loss(lp, length, tours_per_instance=2 * per, beta=0.1).loss
+            loss = loss + amd.clipped_policy_loss(lp, lp, adv).loss
+            ev[2].record()
+            (grad,) = torch.autograd.grad(loss, logits)
+            ev[3].record()
+            torch.cuda.synchronize()
+            return loss, grad, [ev[k].elapsed_time(ev[k + 1]) for k in range(3)]
+
+        learn()
+        t = np.mean(np.array([learn()[2] for _ in range(args.steps)]), axis=0)
+        loss, grad, _ = learn()
+        out["learn"] = {"tours": int(both.shape[0]), "loss": float(loss.detach()), "gradient_finite": bool(grad.isfinite().all()),
+                        "ms": {"tour_log_probs": float(t[0]), "losses": float(t[1]), "gradient": float(t[2]),
+                               "total": float(t.sum())}}
     if args.phases:
         from ml4tspbench_amd import two_opt
         L = _lib.lib()
