@@ -338,7 +338,8 @@ __device__ __forceinline__ void pref_pairs(const PrefParams& p, double (&sum)[2]
             const float against = z >= 0.0f ? e / (1.0f + e) : 1.0f / (1.0f + e);       // sigmoid(-z)
             c[0] += (double)(wins ? p.eps - against : against - p.eps);
             if (wins) {
-                sum[0] += (double)(fmaxf(-z, 0.0f) + log1pf(e) + (p.eps != 0.0f ? p.eps * z : 0.0f));
+                sum[0] += (double)((1.0f - p.eps) * fmaxf(-z, 0.0f) + (p.eps != 0.0f ? p.eps * fmaxf(z, 0.0f) : 0.0f) +
+                                   log1pf(e));
                 sum[1] += 1.0;
             }
         }
@@ -481,8 +482,8 @@ int policy_fill(PolicyParams& p, const void* lp, const void* old, const void* re
     if (rc) return rc;
     if (!(clip_low >= 0.0 && clip_low < 1.0) || !(clip_high >= 0.0))
         return fail(TSP2OPT_E_ARG, "clip_low must be in [0, 1) and clip_high >= 0");
-    if (!(kl_coef >= 0.0) || (kl_coef != 0.0 && !ref))
-        return fail(TSP2OPT_E_ARG, "kl_coef must be >= 0, and 0 without reference log-probabilities");
+    if (!(kl_coef >= 0.0 && kl_coef < __builtin_inf()) || (kl_coef != 0.0 && !ref))
+        return fail(TSP2OPT_E_ARG, "kl_coef must be >= 0 and finite, and 0 without reference log-probabilities");
     if (ratio_of_tour && (!average_of_tours || adv_per_step))
         return fail(TSP2OPT_E_ARG, "ratios of tours are averaged over tours and take one advantage a tour");
     if (!state) return fail(TSP2OPT_E_ARG, "null pointer");
@@ -520,7 +521,8 @@ extern "C" int tsp2opt_policy_loss(const void* logp, const void* old_logp, const
                                    const float* advantages, const uint8_t* mask, float* loss_out, float* stats_out,
                                    void* state, int64_t state_bytes, int64_t num_tours, int64_t steps,
                                    int32_t adv_per_step, int32_t ratio_of_tour, int32_t average_of_tours,
-                                   double clip_low, double clip_high, double kl_coef, int32_t dtype, int32_t device, void* hip_stream)
+                                   double clip_low, double clip_high, double kl_coef, int32_t dtype, int32_t device,
+                                   void* hip_stream)
 {
     PolicyParams p{};
     const int rc = policy_fill(p, logp, old_logp, ref_logp, advantages, mask, num_tours, steps, adv_per_step,
@@ -578,8 +580,8 @@ extern "C" int tsp2opt_preference_loss(const void* logp, const void* ref_logp, c
     if (rc) return rc;
     if (tours_per_instance < 1 || num_tours % tours_per_instance)
         return fail(TSP2OPT_E_ARG, "num_tours % tours_per_instance != 0");
-    if (!(label_smoothing >= 0.0 && label_smoothing < 0.5) || !(beta > 0.0))
-        return fail(TSP2OPT_E_ARG, "beta must be > 0 and label_smoothing in [0, 0.5)");
+    if (!(label_smoothing >= 0.0 && label_smoothing < 0.5) || !(beta > 0.0 && beta < __builtin_inf()))
+        return fail(TSP2OPT_E_ARG, "beta must be > 0 and finite and label_smoothing in [0, 0.5)");
     if (!loss_out || !pairs_out || !state) return fail(TSP2OPT_E_ARG, "null pointer");
     if (num_tours > 0 && (!lengths || (steps > 0 && !logp))) return fail(TSP2OPT_E_ARG, "null pointer");
     const size_t size = element_size(dtype);

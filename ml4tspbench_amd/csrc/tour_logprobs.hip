@@ -283,8 +283,8 @@ __device__ __forceinline__ float scaled_exp(float x)
 
 __device__ __forceinline__ float plain_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// The steps that k_shared cannot see, by a group of lanes: h becomes exp(h - top) of the open entries (positions `at`), 0 of
-// the others; top and the sum.
+// The steps that k_shared cannot see, by a group of lanes: h becomes exp(h - top) of the open entries (positions `at`),
+// 0 of the others; top and the sum.
 template <int K, int G>
 __device__ __forceinline__ void open_terms(float (&h)[K], const float (&at)[K], float when, float& top, float& total)
 {
@@ -347,7 +347,8 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int src)
 
 // Ends the steps of the lanes with `valid`: (tour k, row r, step `when`, node `next` chosen).  A shared total is 2^60 times
 // the sum; steps of which it says nothing are redone one after the other by their group of lanes: all lanes have to be
-// here.  redo(lane, top, total) redoes the step of one of a group's lanes (-1: none).  Returns what the gradient needs to know.
+// here.  redo(lane, top, total) redoes the step of one of a group's lanes (-1: none).  Returns what the gradient needs
+// to know.
 template <typename E, int G, bool SHARED, typename Redo>
 __device__ __forceinline__ float end_steps(const LogpParams& p, bool valid, int64_t map, int64_t k, int r, float when,
                                            int next, float top, float total, int lane, Redo redo)
@@ -428,7 +429,8 @@ __device__ __forceinline__ void open_masks(const Q* at, int l, const Leaves<Q>& 
 #pragma unroll
             for (int r = 0; r < kRows; ++r) {
                 if constexpr (sizeof(Q) == 4) f(r, x, __builtin_amdgcn_fmed3f(y - leaves.t[r], 0.0f, 1.0f));
-                else f(r, x, (float)__builtin_elementwise_min(__builtin_elementwise_max((_Float16)(y - leaves.t[r][0]), (_Float16)0), (_Float16)1));
+                else f(r, x, (float)__builtin_elementwise_min(
+                                 __builtin_elementwise_max((_Float16)(y - leaves.t[r][0]), (_Float16)0), (_Float16)1));
             }
         }
     } else {
@@ -520,7 +522,7 @@ __device__ __forceinline__ void stage_tours(const LogpParams& p, Q* tile, uint16
         for (int c = 0; c < steps; ++c) {
             const int s = c * 64 + lane;
             if (s < p.n && node[c] >= 0) {
-                bad |= (float)tile[q * C + node[c]] != (float)s;       // two steps at one node: one of them sees the other's
+                bad |= (float)tile[q * C + node[c]] != (float)s;       // two steps at one node: one sees the other's
                 after[q * C + node[c]] = (uint16_t)then[c];
             }
         }
@@ -711,26 +713,30 @@ __device__ __forceinline__ void join_equal(int& to, float& g)
         sum += before == to ? x : 0.0f;
         later |= behind == to;
     };
-    step(std::integral_constant<int, 1>()); step(std::integral_constant<int, 2>()); step(std::integral_constant<int, 3>());
-    step(std::integral_constant<int, 4>()); step(std::integral_constant<int, 5>()); step(std::integral_constant<int, 6>());
-    step(std::integral_constant<int, 7>()); step(std::integral_constant<int, 8>()); step(std::integral_constant<int, 9>());
-    step(std::integral_constant<int, 10>()); step(std::integral_constant<int, 11>()); step(std::integral_constant<int, 12>());
-    step(std::integral_constant<int, 13>()); step(std::integral_constant<int, 14>()); step(std::integral_constant<int, 15>());
+    step(std::integral_constant<int, 1>()); step(std::integral_constant<int, 2>());
+    step(std::integral_constant<int, 3>()); step(std::integral_constant<int, 4>());
+    step(std::integral_constant<int, 5>()); step(std::integral_constant<int, 6>());
+    step(std::integral_constant<int, 7>()); step(std::integral_constant<int, 8>());
+    step(std::integral_constant<int, 9>()); step(std::integral_constant<int, 10>());
+    step(std::integral_constant<int, 11>()); step(std::integral_constant<int, 12>());
+    step(std::integral_constant<int, 13>()); step(std::integral_constant<int, 14>());
+    step(std::integral_constant<int, 15>());
     g = sum;
     if (later) to = -1;
 }
 
-// sum_q g_q / S_q [open in tour q] for every entry of a row by the same masked additions, times its exponential, plus g at
-// the chosen entries.  128 maps x 16 tours of 500 nodes in bfloat16: 69 us for 128 MB (27 us at the rate of a large copy), of which
-// 20 are the masked additions and 7 the choices (copies without them take so much less);
-// the rest is reading positions, steps and rows one after the other.
+// sum_q g_q / S_q [open in tour q] for every entry of a row by the same masked additions, times its exponential, plus g
+// at the chosen entries.  128 maps x 16 tours of 500 nodes in bfloat16: 69 us for 128 MB (27 us at the rate of a large
+// copy), of which 20 are the masked additions and 7 the choices (copies without them take so much less); the rest is
+// reading positions, steps and rows one after the other.
 template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
 {
     extern __shared__ float lds[];
     Q* const tile = reinterpret_cast<Q*>(lds);          // [tours of a pass][G K] positions, then [waves][64 K] floats
     __shared__ float4 when[kWaves<G>][kTile][64 / G], weight[kWaves<G>][kTile][64 / G];
-    __shared__ float2 choice[G == 64 ? kWaves<G> : 1][kTile * kRows];     // of the steps: gradient; entry, bit 20: to be redone
+    // of the steps: gradient; entry, bit 20: to be redone
+    __shared__ float2 choice[G == 64 ? kWaves<G> : 1][kTile * kRows];
     const SharedWork<K, G> w(p);
     const int lane = w.lane, l = w.l;
     const bool once = G == 64 && p.per <= kTile;        // 16 lanes a row: the four rows' choices at one go
@@ -751,7 +757,9 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         if (want_to && s.g != 0.0f) s.to = (int)p.next[k * p.n + i];
         return s;
     };
-    auto unseen = [](const Step& s) { return s.g != 0.0f && (!(s.total >= kSmall) || !(fabsf(s.g / s.total) < kInf)); };
+    // g over the sum itself, without its 2^60: small gradients keep their digits
+    auto weight_of = [](const Step& s) { return (s.g * 0x1p30f) / (s.total * 0x1p-30f); };
+    auto unseen = [&](const Step& s) { return s.g != 0.0f && (!(s.total >= kSmall) || !(fabsf(weight_of(s)) < 0x1p100f)); };
 
     float sum[kRows][K];
 #pragma unroll
@@ -770,7 +778,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
             any_redo |= redo;
             if (once) choice[w.wave][x] = make_float2(s.g, __int_as_float(redo ? s.to | 1 << 20 : s.to));
             reinterpret_cast<float*>(when[w.wave])[x] = pack_step<Q>(s.t);
-            reinterpret_cast<float*>(weight[w.wave])[x] = redo || s.g == 0.0f ? 0.0f : s.g / s.total;
+            reinterpret_cast<float*>(weight[w.wave])[x] = redo || s.g == 0.0f ? 0.0f : weight_of(s);
         }
         __syncthreads();
         for (int q = 0; q < count; ++q) {
@@ -811,7 +819,10 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         const float from = base_of(p.top[w.map * p.n + min(i, p.n - 1)]);
         // an entry that no tour had open may hold anything: its weight is 0, and so is its gradient
 #pragma unroll
-        for (int x = 0; x < K; ++x) d[x] = sum[r][x] != 0.0f ? -sum[r][x] * scaled_exp(h[x] - from) : 0.0f;
+        for (int x = 0; x < K; ++x) {
+            const float y = plain_exp(0.5f * (h[x] - from));        // the square would be flushed too soon
+            d[x] = sum[r][x] != 0.0f ? -(sum[r][x] * y) * y : 0.0f;
+        }
 #pragma unroll
         for (int x = 0; x < K; ++x) hits[column<K, G>(x, l)] = 0.0f;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the lanes of a group write each other's columns
@@ -1087,7 +1098,8 @@ inline int parts_of(int n) { return (n + 64 * kMaxPer - 1) / (64 * kMaxPer); }
 
 inline int held(int n)
 {
-    const int lanes = n <= kShortRow ? 16 : 64, parts = parts_of(n), need = ((n + parts - 1) / parts + lanes - 1) / lanes;
+    const int lanes = n <= kShortRow ? 16 : 64, parts = parts_of(n);
+    const int need = ((n + parts - 1) / parts + lanes - 1) / lanes;
     for (int k : {1, 2, 4, 6, 8, 12})
         if (need <= k) return k;
     return kMaxPer;
@@ -1243,6 +1255,7 @@ extern "C" int64_t tsp2opt_tour_logprobs_state_bytes(int64_t num_tours, int32_t 
                               4);
     if (rc) return rc;
     if (num_tours < 0 || num_tours % tours_per_map) return fail(TSP2OPT_E_ARG, "bad size");
+    if (num_tours > 0x7fffffffll) return fail(TSP2OPT_E_UNSUPPORTED, "too many tours");
     return LogpState(num_tours, n, tours_per_map, rows).bytes;
 }
 
@@ -1255,7 +1268,8 @@ extern "C" int tsp2opt_tour_logprobs(const void* logits, const int64_t* tours, f
                               dtype, 4);
     if (rc) return rc;
     if (num_tours == 0 || n == 1) return 0;
-    if (state_bytes < LogpState(num_tours, n, tours_per_map, rows).bytes) return fail(TSP2OPT_E_WORKSPACE, "state_bytes too small");
+    if (state_bytes < LogpState(num_tours, n, tours_per_map, rows).bytes)
+        return fail(TSP2OPT_E_WORKSPACE, "state_bytes too small");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(TSP2OPT_E_HIP, "hipSetDevice failed");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
@@ -1288,7 +1302,8 @@ extern "C" int tsp2opt_tour_logprobs_grad(const void* logits, const int64_t* tou
     if (!grad_logp) return fail(TSP2OPT_E_ARG, "null pointer");
     if (reinterpret_cast<uintptr_t>(grad_logp) % 4)
         return fail(TSP2OPT_E_ARG, "misaligned pointer (arrays must be aligned to their element size)");
-    if (state_bytes < LogpState(num_tours, n, tours_per_map, rows).bytes) return fail(TSP2OPT_E_WORKSPACE, "state_bytes too small");
+    if (state_bytes < LogpState(num_tours, n, tours_per_map, rows).bytes)
+        return fail(TSP2OPT_E_WORKSPACE, "state_bytes too small");
     DeviceGuard guard(device);
     if (!guard.ok) return fail(TSP2OPT_E_HIP, "hipSetDevice failed");
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);

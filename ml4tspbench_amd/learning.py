@@ -11,6 +11,7 @@ csrc/learning_ext.cpp.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -123,8 +124,8 @@ def clipped_policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, ad
         raise ValueError("advantages must be (T,), or (T, steps) with ratios of steps")
     if not advantages.dtype.is_floating_point:
         raise TypeError(f"advantages must be floating point, got {advantages.dtype}")
-    if not (0.0 <= clip_low < 1.0 and clip_high >= 0.0 and kl_coef >= 0.0):
-        raise ValueError("clip_low must be in [0, 1), clip_high and kl_coef >= 0")
+    if not (0.0 <= clip_low < 1.0 and clip_high >= 0.0 and 0.0 <= kl_coef < math.inf):
+        raise ValueError("clip_low must be in [0, 1), clip_high and kl_coef >= 0, kl_coef finite")
     if kl_coef and ref_log_probs is None:
         raise ValueError("kl_coef needs ref_log_probs")
     _same_device(log_probs, "log_probs and the other arrays", old_log_probs, advantages, ref_log_probs, mask)
@@ -152,7 +153,8 @@ def preference_loss(log_probs: torch.Tensor, lengths: torch.Tensor, *, tours_per
     lengths differ (``pairs="best"``: only those with the instance's first shortest tour) the loss is the average of
     ``-(1 - label_smoothing) log sigmoid(s_short - s_long) - label_smoothing log sigmoid(s_long - s_short)``.
     Sampled tours against the same tours after ``two_opt_device``: stack them as an instance's tours.  NaN lengths are
-    in no pair; without any pair the loss is 0.  Asynchronous on the current stream."""
+    in no pair; without any pair the loss is 0.  Steps of -inf (forbidden edges) make a tour's score -inf and two such
+    tours' pair NaN: mask them, or mark forbidden edges by a finite logit.  Asynchronous on the current stream."""
     _step_arrays(log_probs, mask, ref_log_probs=ref_log_probs)
     per = int(tours_per_instance)
     T = log_probs.shape[0]
@@ -162,8 +164,8 @@ def preference_loss(log_probs: torch.Tensor, lengths: torch.Tensor, *, tours_per
         raise TypeError(f"lengths must be float32 or float64, got {lengths.dtype}")
     if pairs not in ("all", "best"):
         raise ValueError(f"pairs must be 'all' or 'best', got {pairs!r}")
-    if not (beta > 0.0 and 0.0 <= label_smoothing < 0.5):
-        raise ValueError("beta must be > 0 and label_smoothing in [0, 0.5)")
+    if not (0.0 < beta < math.inf and 0.0 <= label_smoothing < 0.5):
+        raise ValueError("beta must be > 0 and finite and label_smoothing in [0, 0.5)")
     _same_device(log_probs, "log_probs and the other arrays", lengths, ref_log_probs, mask)
     return PreferenceLossResult(*_lib.learning_ext().preference_loss(
         log_probs, ref_log_probs, lengths, mask, per, pairs == "best", bool(per_step), beta, label_smoothing))

@@ -216,6 +216,8 @@ def test_argument_checks_without_gpu():
         (ValueError, "'all' or 'best'", lambda: amd.preference_loss(lp, length, tours_per_instance=2, pairs="worst")),
         (ValueError, "beta", lambda: amd.preference_loss(lp, length, tours_per_instance=2, beta=0.0)),
         (ValueError, "beta", lambda: amd.preference_loss(lp, length, tours_per_instance=2, label_smoothing=0.5)),
+        (ValueError, "beta", lambda: amd.preference_loss(lp, length, tours_per_instance=2, beta=math.inf)),
+        (ValueError, "kl_coef", lambda: amd.clipped_policy_loss(lp, lp, adv, ref_log_probs=lp, kl_coef=math.inf)),
         (ValueError, "same HIP device", lambda: amd.preference_loss(lp, length, tours_per_instance=2)),
     ]:
         with pytest.raises(exc, match=what):
@@ -263,6 +265,8 @@ def test_c_abi_checks_without_gpu():
 
     assert L.tsp2opt_preference_loss_state_bytes(-1) == -1
     assert pref(per=0) == -1 and pref(per=3) == -1 and pref(beta=0.0) == -1 and pref(eps=0.5) == -1 and pref(dt=1) == -1
+    assert pref(beta=math.inf) == -1 and policy(kl=math.inf, ref=at) == -1
+    assert L.tsp2opt_tour_logprobs_state_bytes(1 << 60, 10, 2, 0) == -2
     assert pref(lp=None) == -1 and pref(ln=None) == -1 and pref(ln=at2) == -1 and pref(pairs=None) == -1
     assert pref(nbytes=8) == -3 and pref(S=1 << 32) == -2
     assert L.tsp2opt_preference_loss_grad(None, at, 1 << 30, None, at, 4, 6, 0, 0, None) == -1
@@ -432,6 +436,24 @@ def test_gpu_log_probs_gradient_against_differences(per, n):
         size = float(g.abs().sum())
         tol = 8 * U * 30 * size / step + step ** 2 / 6 * 8 * size
         assert abs(float((f[0] - f[1]) / (2 * step) - (grad.double() * way).sum())) < tol
+
+
+@gpu
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -60, 2.0 ** 40, 2.0 ** 90])
+@pytest.mark.parametrize("per,n", [(1, 40), (3, 40), (3, 300), (20, 300), (2, 1100), (2, 2100)])
+def test_gpu_log_probs_gradients_of_any_size(per, n, size):
+    """Incoming gradients far from 1 (a saturated preference loss sends such): a power of two passes through exactly,
+    entries of 2^-20 of it and more stay normal numbers."""
+    import ml4tspbench_amd as amd
+    gen = torch.Generator().manual_seed(n + per)
+    tours = make_tours(gen, per, n)
+    h = torch.rand((1, n, n), generator=gen)
+    g = torch.randn((per, n - 1), generator=gen)
+    x = h.cuda().requires_grad_()
+    lp = amd.tour_log_probs(x, tours.cuda(), tours_per_map=per)
+    (grad,) = torch.autograd.grad(lp, x, g.cuda() * size)
+    _, _, want, tol = ref_log_probs(h, tours, per, "node", g)
+    compare("gradient", grad.double().cpu() / size, want, tol)
 
 
 @gpu
@@ -608,6 +630,12 @@ def test_gpu_preference_loss_edges():
     a = amd.preference_loss(lp, torch.tensor([1.0, 2, 3, 4]).cuda(), tours_per_instance=2)
     b = amd.preference_loss(lp, torch.tensor([1.0, 2, 3, 4], dtype=torch.float64).cuda(), tours_per_instance=2)
     assert torch.equal(a.loss, b.loss) and int(a.num_pairs) == 2
+    never = torch.tensor([[-math.inf], [1.0], [2.0], [-math.inf]], device="cuda", requires_grad=True)
+    for order, eps, want in (([1.0, 2, 2, 1], 0.0, math.inf), ([2.0, 1, 1, 2], 0.0, 0.0), ([1.0, 2, 2, 1], 0.1, math.inf),
+                             ([2.0, 1, 1, 2], 0.1, math.inf)):
+        res = amd.preference_loss(never, torch.tensor(order).cuda(), tours_per_instance=2, label_smoothing=eps)
+        assert float(res.loss.detach()) == want
+        assert torch.autograd.grad(res.loss, never)[0].isfinite().all()
     far = torch.tensor([[-300.0], [300.0], [200.0], [-200.0]])
     check_preference(far, torch.tensor([1.0, 2, 1, 2]), 2, None, None, 1.0, 0.0, "all", False)
     for shape in ((0, 3), (4, 0)):
