@@ -574,7 +574,8 @@ struct SharedWork {
 // run their phases side by side and overlap little.  Measured and left out: 6 instead of 4 waves a SIMD by limiting the
 // registers (the same), workgroups of four waves (53 and 65 us), several blocks of rows in a workgroup with the next one's
 // rows in flight (62 and 70 us: its registers halve the waves), sums over the lanes by v_mfma_f32_16x16x4 with a unit
-// matrix (64 us in bfloat16 against 51: the matrix and vector instructions of these kernels do not run side by side).
+// matrix (64 us in bfloat16 against 51: the matrix and vector instructions of these kernels do not run side by side),
+// positions kept in memory as half floats in the order of the tile (62 and 54 us: nothing waits for them).
 template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 {
