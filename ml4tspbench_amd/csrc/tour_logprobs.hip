@@ -105,6 +105,17 @@ struct Pack<E, 1> {
     typedef E type;
 };
 
+// V adjacent entries of a row in LDS, aligned to their size: one access of 8 or 16 bytes a lane.  (Two of 4 bytes would
+// leave every other bank idle.)
+template <typename E, int V>
+struct Aligned {
+    typedef E type __attribute__((ext_vector_type(V)));
+};
+template <typename E>
+struct Aligned<E, 1> {
+    typedef E type;
+};
+
 // Loads are issued without a branch: a lane at or behind the end reads the row's last V entries instead (in front of a
 // short last part there is the previous one) and end_row puts its entries in place.
 template <typename E, int K>
@@ -422,26 +433,33 @@ template <int K, int G, typename Q, typename F>
 __device__ __forceinline__ void open_masks(const Q* at, int l, const Leaves<Q>& leaves, F f)
 {
     constexpr int V = kVec<K>;
-    if constexpr (sizeof(Q) == 4 || V == 1) {
+    if constexpr (V == 1) {                             // half floats always: one entry a lane is a row of up to 16
+        const Q y = at[l];
 #pragma unroll
-        for (int x = 0; x < K; ++x) {
-            const Q y = at[column<K, G>(x, l)];
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                if constexpr (sizeof(Q) == 4) f(r, x, __builtin_amdgcn_fmed3f(y - leaves.t[r], 0.0f, 1.0f));
-                else f(r, x, (float)__builtin_elementwise_min(
-                                 __builtin_elementwise_max((_Float16)(y - leaves.t[r][0]), (_Float16)0), (_Float16)1));
-            }
-        }
+        for (int r = 0; r < kRows; ++r)
+            f(r, 0, (float)__builtin_elementwise_min(
+                        __builtin_elementwise_max((_Float16)(y - leaves.t[r][0]), (_Float16)0), (_Float16)1));
     } else {
 #pragma unroll
-        for (int x = 0; x < K; x += 2) {
-            const half2 y = *reinterpret_cast<const half2*>(at + column<K, G>(x, l));
+        for (int c = 0; c < K; c += V) {
+            const auto y = *reinterpret_cast<const typename Aligned<Q, V>::type*>(at + column<K, G>(c, l));
+            if constexpr (sizeof(Q) == 4) {
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) {
-                const half2 m = __builtin_elementwise_min(__builtin_elementwise_max(y - leaves.t[r], (half2)0), (half2)1);
-                f(r, x, (float)m[0]);
-                f(r, x + 1, (float)m[1]);
+                for (int v = 0; v < V; ++v)
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) f(r, c + v, __builtin_amdgcn_fmed3f(y[v] - leaves.t[r], 0.0f, 1.0f));
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; v += 2) {
+                    const half2 two = {y[v], y[v + 1]};
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r) {
+                        const half2 m = __builtin_elementwise_min(__builtin_elementwise_max(two - leaves.t[r], (half2)0),
+                                                                  (half2)1);
+                        f(r, c + v, (float)m[0]);
+                        f(r, c + v + 1, (float)m[1]);
+                    }
+                }
             }
         }
     }
@@ -467,9 +485,15 @@ __device__ __forceinline__ void stage(Q* tile, const float* pos, int count, int 
             float at[K];
             end_row<float, K, 64>(raw[a], lane, cols, at);
 #pragma unroll
-            for (int c = 0; c < K / V; ++c)
+            for (int c = 0; c < K / V; ++c) {
+                typename Aligned<Q, V>::type y;
 #pragma unroll
-                for (int v = 0; v < V; ++v) tile[q * C + c * 64 * V + lane * V + v] = (Q)at[c * V + v];
+                for (int v = 0; v < V; ++v) {
+                    if constexpr (V == 1) y = (Q)at[c];
+                    else y[v] = (Q)at[c * V + v];
+                }
+                *reinterpret_cast<typename Aligned<Q, V>::type*>(tile + q * C + c * 64 * V + lane * V) = y;
+            }
         }
     } else {
         constexpr int steps = (C + 63) / 64;
@@ -579,7 +603,7 @@ struct SharedWork {
 template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared(LogpParams p)
 {
-    extern __shared__ float lds[];
+    extern __shared__ __align__(16) float lds[];
     Q* const tile = reinterpret_cast<Q*>(lds);          // [tours of a pass][G K] positions
     __shared__ float4 when[kWaves<G>][kTile][64 / G];   // the steps at which the tours leave a wave's rows
     __shared__ uint16_t after[G == 16 ? kTile * 16 * K : 1];
@@ -727,13 +751,13 @@ __device__ __forceinline__ void join_equal(int& to, float& g)
 }
 
 // sum_q g_q / S_q [open in tour q] for every entry of a row by the same masked additions, times its exponential, plus g
-// at the chosen entries.  128 maps x 16 tours of 500 nodes in bfloat16: 69 us for 128 MB (27 us at the rate of a large
+// at the chosen entries.  128 maps x 16 tours of 500 nodes in bfloat16: 66 us for 128 MB (27 us at the rate of a large
 // copy), of which 20 are the masked additions and 7 the choices (copies without them take so much less); the rest is
 // reading positions, steps and rows one after the other.
 template <typename E, int K, int G, typename Q>
 __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
 {
-    extern __shared__ float lds[];
+    extern __shared__ __align__(16) float lds[];
     Q* const tile = reinterpret_cast<Q*>(lds);          // [tours of a pass][G K] positions, then [waves][64 K] floats
     __shared__ float4 when[kWaves<G>][kTile][64 / G], weight[kWaves<G>][kTile][64 / G];
     // of the steps: gradient; entry, bit 20: to be redone
@@ -810,6 +834,8 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         join_equal(mine.to, mine.g);
     }
     const bool redo_any = __any(any_redo);
+    constexpr int V = kVec<K>;
+    using Hits = typename Aligned<float, V>::type;
     float* const hits = reinterpret_cast<float*>(tile + min(kTile, p.per) * G * K) + (w.wave * (64 / G) + w.group) * G * K;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -825,7 +851,7 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
             d[x] = sum[r][x] != 0.0f ? -(sum[r][x] * y) * y : 0.0f;
         }
 #pragma unroll
-        for (int x = 0; x < K; ++x) hits[column<K, G>(x, l)] = 0.0f;
+        for (int x = 0; x < K; x += V) *reinterpret_cast<Hits*>(hits + column<K, G>(x, l)) = Hits(0.0f);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the lanes of a group write each other's columns
         constexpr int at_once = G == 64 ? 64 : 16;
         for (int q0 = 0; q0 < p.per; q0 += at_once) {
@@ -877,7 +903,14 @@ __global__ __launch_bounds__(64 * kWaves<G>) void k_shared_grad(LogpParams p)
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int x = 0; x < K; ++x) d[x] += hits[column<K, G>(x, l)];
+        for (int x = 0; x < K; x += V) {
+            const Hits y = *reinterpret_cast<const Hits*>(hits + column<K, G>(x, l));
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if constexpr (V == 1) d[x] += y;
+                else d[x + v] += y[v];
+            }
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (G == 64 || i < p.n)
             store_row<E, K, G>(static_cast<E*>(p.grad) + (w.map * p.n + i) * (int64_t)p.n + w.col0, l, w.cols, d);
