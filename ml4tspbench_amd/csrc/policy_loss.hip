@@ -597,6 +597,7 @@ extern "C" int tsp2opt_preference_loss(const void* logp, const void* ref_logp, c
     p.per = tours_per_instance; p.best = best_only; p.per_step = per_step; p.beta = beta; p.eps = (float)label_smoothing;
     p.loss = loss_out; p.pairs = pairs_out;
     pref_state(p, state);
+    // one workgroup does all: it has 8 threads a tour, so the pairs of 512 tours take four turns of it
     if (num_tours * steps <= kOneBlock && num_tours <= 512 && tours_per_instance <= 64) {
         const Shape s = shape_of(num_tours, steps, true);
         T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_pref_one<E, G>), dim3(1), dim3(kOneThreads), 0,
@@ -605,6 +606,8 @@ extern "C" int tsp2opt_preference_loss(const void* logp, const void* ref_logp, c
         const Shape s = shape_of(num_tours, steps, false);
         T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_pref_rows<E, G>), dim3(s.grid), dim3(s.threads), 0,
                                                                      stream, p)));
+        // us with 8 and with 64 threads a tour, instances x tours: 2000 x 16 6.5, 15.5; 500 x 64 13.5, 16.3; 250 x 128 21.7,
+        // 23.8; 10 x 1000 78, 42.5
         const int w = tours_per_instance <= 64 ? 8 : 64;
         const int64_t need = (num_tours * w + 255) / 256;
         const unsigned blocks = (unsigned)(need < kMaxBlocks ? need : kMaxBlocks);
