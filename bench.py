@@ -51,7 +51,7 @@ CONFIGS = {
 FLOP_PER_PAIR = 15.0          # 2 x (2 sub + 2 mul + add + sqrt) + 3 add/sub
 PEAK_FP32_VALU_TFLOPS = 157.3  # MI355X_MICROARCH.md: 256 CU x 2.4 GHz x 256 FLOP/clk/CU
 PEAK_FP64_VALU_TFLOPS = 78.6   # SURVEY.md 8(d3) / BASELINE.md: the fp64 vector peak
-# DESIGN.md 4.2 (tools/valu_chain_microbench.hip): SIMD cycles per 64 evaluated pairs of the scalar
+# tools/valu_chain_microbench.hip: SIMD cycles per 64 evaluated pairs of the scalar
 # per-pair chain (1 v_sqrt_f32, sub / mul / fma / add, min) -- the instruction floor of the sweep; the build uses no
 # packed FP32 instructions
 INSN_FLOOR_CYCLES_PER_64_PAIRS = 37.5

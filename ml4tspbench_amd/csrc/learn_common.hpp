@@ -1,4 +1,4 @@
-// ml4tspbench_amd/csrc/learn_common.hpp -- element types and wave sums shared by the learning operators
+// ml4tspbench_amd/csrc/learn_common.hpp -- element types shared by the learning operators
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -28,19 +28,6 @@ __device__ __forceinline__ T narrow(float x)
 inline int element_size(int dtype)
 {
     return dtype == TSP2OPT_DTYPE_F32 ? 4 : (dtype == TSP2OPT_DTYPE_BF16 || dtype == TSP2OPT_DTYPE_F16) ? 2 : 0;
-}
-
-template <typename V>
-__device__ __forceinline__ V wave_sum(V v)
-{
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-
-__device__ __forceinline__ float wave_max(float v)
-{
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
 }
 
 #define T2O_BY_DTYPE(dtype, CALL)                                  \

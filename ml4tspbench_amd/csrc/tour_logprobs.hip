@@ -1160,7 +1160,10 @@ struct LogpShape {
         k = held(n);
         parts = parts_of(n);
         tours = per < kTile ? per : kTile;
-        position_threads = n <= 64 ? 64 : n <= 128 ? 128 : n <= 1024 ? 256 : 1024;
+        // us of k_positions with 64, 128, 256, 512, 1024 threads: 20000 tours of 50 nodes 11, 15.5, 24, 42, 71; 10000 of 100
+        // 9.4, 10.2, 15, 25, 42; 2048 of 500 10.7, 7.6, 6.5, 7.8, 11.6; 128 of 1000 15, 8.7, 5.8, 4.8, 4.8; 16 of 10000
+        // 131, 68, 36, 20, 14
+        position_threads = n <= 128 ? 64 : n <= 512 ? 256 : n <= 1024 ? 512 : 1024;
         const int64_t maps = T / per;
         if (per > 1) {
             const int block = n <= kShortRow ? kWaves<16> * kWaveRows<16> : kWaves<64> * kWaveRows<64>;
