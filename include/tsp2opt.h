@@ -293,7 +293,8 @@ int tsp2opt_tour_logprobs_grad(const void* logits, const int64_t* tours, const v
  *   term = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(d) - 1 - d with d = ref_logp - logp per step,
  *   loss = average(term) + kl_coef * average(kl)
  *   average_of_tours 0: over all kept steps; 1: over a tour's kept steps, then over the tours that have any
- *   ref_logp  NULL: no KL term (kl_coef must be 0, else finite);  advantages (num_tours) or, adv_per_step, (num_tours, steps) float
+ *   ref_logp  NULL: no KL term (kl_coef must be 0, else finite)
+ *   advantages (num_tours) or, adv_per_step, (num_tours, steps) float
  *   mask      (num_tours, steps) bytes, 0 = step does not count and its values are not used; NULL: all count
  *   loss_out  1 float; stats_out 2 floats: average kl, share of clipped steps (tours).  Nothing kept: all 0
  * tsp2opt_policy_loss_grad -- grad_out (num_tours, steps) in `dtype` = grad_loss[0] * d loss / d logp, 0 at steps that
@@ -316,7 +317,8 @@ int tsp2opt_policy_loss_grad(const void* logp, const void* old_logp, const void*
  *   s = beta * sum over kept steps of (logp - ref_logp) (per_step: their mean), and over all pairs (a, b) of tours of
  *   one instance with lengths[a] < lengths[b] (best_only: a = the instance's first shortest tour only) the average of
  *   -(1 - label_smoothing) log sigmoid(s_a - s_b) - label_smoothing log sigmoid(s_b - s_a)
- *   beta > 0 and finite;  lengths (num_tours) double, as tsp2opt_evaluate writes them; equal lengths are no pair, NaN is in none
+ *   beta > 0 and finite;  lengths (num_tours) double, as tsp2opt_evaluate writes them; equal lengths are no pair, NaN
+ *   is in none
  *   ref_logp, mask  as above, or NULL;  loss_out 1 float, pairs_out 1 int64.  No pair: loss 0
  * tsp2opt_preference_loss_grad -- grad_out (num_tours, steps) in `dtype` = grad_loss[0] * d loss / d logp.
  */
