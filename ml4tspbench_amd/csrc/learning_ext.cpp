@@ -10,6 +10,7 @@
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <memory>
@@ -79,13 +80,17 @@ Tensor one(const Maybe& x) { return x ? *x : Tensor(); }
 // captured graphs never share it.
 Tensor state_like(const Tensor& x, int64_t bytes) { return at::empty({bytes}, x.options().dtype(at::kByte)); }
 
-// The kernels have no second derivative: asking for it raises instead of treating the gradient as a constant.
-Tensor once(Tensor grad)
+// The kernels have no second derivative: with create_graph the gradient's own node is one that raises when it is reached,
+// instead of the gradient being a constant.  It has the edges of the operator's inputs and of the incoming gradients, so
+// that a derivative of an expression which mixes the gradient with others meets it on its way to any of them.
+Tensor once(Tensor grad, const variable_list& incoming)
 {
     if (!c10::GradMode::is_enabled()) return grad;
-    auto node = std::make_shared<torch::autograd::DelayedError>(
-        "the learning operators have no second derivative", 1);
-    return node->apply({grad})[0];
+    auto edges = torch::autograd::get_current_node()->next_edges();
+    for (auto& edge : torch::autograd::collect_next_edges(incoming)) edges.push_back(std::move(edge));
+    torch::autograd::set_history(grad, std::make_shared<torch::autograd::Error>(
+                                           "the learning operators have no second derivative", std::move(edges)));
+    return grad;
 }
 
 struct LogProbs : public Function<LogProbs> {
@@ -112,13 +117,13 @@ struct LogProbs : public Function<LogProbs> {
         const auto how = ctx->saved_data["how"].toIntVector();
         const int64_t T = tours.size(0), n = tours.size(1) - 1;
         Tensor grad = at::empty(logits.sizes(), logits.options());
-        if (n == 1) return {once(grad.zero_()), Tensor(), Tensor(), Tensor()};
+        if (n == 1) return {once(grad.zero_(), grads), Tensor(), Tensor(), Tensor()};
         const Tensor g = grads[0].to(at::kFloat).contiguous();
         checked(api.logp_grad(ptr(logits), ptr<int64_t>(tours), ptr(state), state.numel(), ptr<float>(g), ptr(grad), T,
                               (int)n, (int)how[0], (int)how[1], logits.stride(0), logits.stride(1), code_of(logits),
                               logits.get_device(), stream_of(logits)),
                 "tsp2opt_tour_logprobs_grad");
-        return {once(grad), Tensor(), Tensor(), Tensor()};
+        return {once(grad, grads), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -160,7 +165,7 @@ struct PolicyLoss : public Function<PolicyLoss> {
                                 saved[3].dim() == 2, (int)mode[0], (int)mode[1], how[0], how[1], how[2], code_of(lp),
                                 lp.get_device(), stream_of(lp)),
                 "tsp2opt_policy_loss_grad");
-        none[0] = once(grad);
+        none[0] = once(grad, grads);
         return none;
     }
 };
@@ -198,7 +203,7 @@ struct PreferenceLoss : public Function<PreferenceLoss> {
         checked(api.pref_grad(ptr<uint8_t>(saved[0]), ptr(state), state.numel(), ptr<float>(g), ptr(grad), like[0], like[1],
                               code_of(grad), state.get_device(), stream_of(state)),
                 "tsp2opt_preference_loss_grad");
-        none[0] = once(grad);
+        none[0] = once(grad, grads);
         return none;
     }
 };

@@ -769,6 +769,37 @@ def test_gpu_second_derivative_and_changed_input_are_refused():
 
 
 @gpu
+@pytest.mark.parametrize("op", ["log_probs", "log_probs_strided", "policy", "preference", "one_node"])
+def test_gpu_second_derivatives_raise_and_are_not_dropped(op):
+    """With create_graph the gradient requires grad, and whatever derivative needs its own raises: alone, mixed with the
+    operator's value (as a gradient penalty is), by backward() and by grad() in the leaf or in the incoming gradient."""
+    import ml4tspbench_amd as amd
+    heat, tours, old, adv, length, per = step_inputs(7, M=2, per=2, n=20)
+    x = (heat if op.startswith("log") else torch.zeros((3, 1, 1), device="cuda") if op == "one_node" else old.detach()
+         ).clone().requires_grad_()
+
+    def value(x):
+        if op == "policy":
+            return amd.clipped_policy_loss(x, old, adv).loss
+        if op == "preference":
+            return amd.preference_loss(x, length, tours_per_instance=per).loss
+        if op == "one_node":
+            return amd.tour_log_probs(x, torch.zeros((3, 2), dtype=torch.int64, device="cuda")).sum()
+        return amd.tour_log_probs(x.transpose(1, 2) if op.endswith("strided") else x, tours, tours_per_map=per).sum()
+
+    weight = torch.ones((), device="cuda", requires_grad=True)
+    (plain,) = torch.autograd.grad(value(x), x)
+    for ask in (lambda g: torch.autograd.grad(value(x) + g.pow(2).sum(), x), lambda g: g.sum().backward(),
+                lambda g: (value(x) + g.pow(2).sum()).backward(), lambda g: torch.autograd.grad(g.sum() + weight, weight)):
+        (g,) = torch.autograd.grad(value(x) * weight, x, create_graph=True)
+        assert g.requires_grad and torch.equal(g.detach(), plain) and not plain.requires_grad
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            ask(g)
+    (g,) = torch.autograd.grad(value(x) * weight, x, create_graph=True)         # not reached: nothing raises
+    assert torch.equal(torch.autograd.grad(value(x) + g.detach().sum(), x)[0], plain)
+
+
+@gpu
 def test_gpu_run_of_decoder_two_opt_evaluation_and_losses():
     """As they are used: tours of heat maps are scored, improved, measured, and the losses' gradient comes back to the
     maps; every value against the formulas, chained in 64 bits on the CPU."""
