@@ -40,19 +40,18 @@ struct Api {
     decltype(&tsp2opt_preference_loss_grad) pref_grad;
 } api;
 
-struct Failure : std::runtime_error {       // Tsp2optError where it reaches Python
-    using std::runtime_error::runtime_error;
-};
+PyObject* failure_class = nullptr;          // Tsp2optError
 
-PyObject* failure_class = nullptr;
-
+// What _lib.check() raises.  Autograd's device thread calls this too: it holds no interpreter lock, and the exception
+// reaches the caller of backward() as it is.
 int64_t checked(int64_t rc, const char* what)
 {
-    if (rc < 0) {
-        const char* msg = api.last_error();
-        throw Failure(std::string(what) + " failed (" + std::to_string(rc) + "): " + (msg ? msg : ""));
-    }
-    return rc;
+    if (rc >= 0) return rc;
+    const char* msg = api.last_error();
+    const std::string text = std::string(what) + " failed (" + std::to_string(rc) + "): " + (msg ? msg : "");
+    py::gil_scoped_acquire gil;
+    PyErr_SetObject(failure_class, py::handle(failure_class)(text, rc).ptr());
+    throw py::error_already_set();
 }
 
 int code_of(const Tensor& x)
@@ -217,13 +216,6 @@ Maybe constant(const Maybe& x) { return x ? Maybe(x->detach().contiguous()) : x;
 
 PYBIND11_MODULE(_learning_ext, m)
 {
-    py::register_exception_translator([](std::exception_ptr p) {
-        try {
-            if (p) std::rethrow_exception(p);
-        } catch (const Failure& e) {
-            PyErr_SetString(failure_class, e.what());
-        }
-    });
     m.def("bind", [](const std::vector<uintptr_t>& at, py::object error) {
         failure_class = error.release().ptr();
         if (at.size() != 10) throw std::runtime_error("bind: ten entry points");

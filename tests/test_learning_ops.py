@@ -273,6 +273,18 @@ def test_c_abi_checks_without_gpu():
     assert L.tsp2opt_preference_loss_grad(None, at, 8, at, at, 4, 6, 0, 0, None) == -3
 
 
+def test_errors_of_the_library_keep_their_code():
+    """Tsp2optError.code is the library's return code, as for the operators that call it through _lib.check()."""
+    from ml4tspbench_amd import _lib
+    ext = _lib.learning_ext()
+    with pytest.raises(_lib.Tsp2optError, match="65535") as e:
+        ext.tour_log_probs(torch.zeros(1, 2, 2), torch.zeros((1, 70001), dtype=torch.int64), 1, 0)
+    assert e.value.code == _lib.E_UNSUPPORTED
+    with pytest.raises(_lib.Tsp2optError, match="bad size") as e:
+        ext.tour_log_probs(torch.zeros(1, 2, 2), torch.zeros((3, 11), dtype=torch.int64), 2, 0)
+    assert e.value.code == _lib.E_ARG
+
+
 def test_reference_gradient_matches_differences():
     """The formula the kernels are held to, against central differences in 64 bits."""
     gen = torch.Generator().manual_seed(3)
@@ -797,6 +809,17 @@ def test_gpu_second_derivatives_raise_and_are_not_dropped(op):
             ask(g)
     (g,) = torch.autograd.grad(value(x) * weight, x, create_graph=True)         # not reached: nothing raises
     assert torch.equal(torch.autograd.grad(value(x) + g.detach().sum(), x)[0], plain)
+
+
+@gpu
+def test_gpu_refusals_of_the_library_keep_their_code():
+    import ml4tspbench_amd as amd
+    from ml4tspbench_amd import _lib
+    n = 70000                                               # rows that share their memory
+    heat = torch.zeros(n, device="cuda").as_strided((1, n, n), (0, 0, 1)).requires_grad_()
+    with pytest.raises(_lib.Tsp2optError, match="65535") as e:
+        amd.tour_log_probs(heat, torch.arange(n + 1, device="cuda")[None])
+    assert e.value.code == _lib.E_UNSUPPORTED
 
 
 @gpu
