@@ -13,6 +13,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
+#include <limits>
 #include <memory>
 #include <optional>
 #include <string>
@@ -93,12 +95,12 @@ Tensor once(Tensor grad, const variable_list& incoming)
 }
 
 struct LogProbs : public Function<LogProbs> {
-    static Tensor forward(AutogradContext* ctx, Tensor logits, const Tensor& tours, int64_t per, int64_t rows)
+    static Tensor forward(AutogradContext* ctx, Tensor logits, const Tensor& tours, int64_t per, int64_t rows,
+                          int64_t state_bytes)
     {
         const int64_t T = tours.size(0), n = tours.size(1) - 1;
         if (n > 1 && logits.stride(2) != 1) logits = logits.contiguous();
-        Tensor state = state_like(logits, checked(api.logp_bytes(T, (int)n, (int)per, (int)rows),
-                                                  "tsp2opt_tour_logprobs_state_bytes"));
+        Tensor state = state_like(logits, state_bytes);
         Tensor out = at::empty({T, n - 1}, logits.options().dtype(at::kFloat));
         checked(api.logp(ptr(logits), ptr<int64_t>(tours), ptr<float>(out), ptr(state), state.numel(), T, (int)n, (int)per,
                          (int)rows, logits.stride(0), logits.stride(1), code_of(logits), logits.get_device(),
@@ -116,13 +118,13 @@ struct LogProbs : public Function<LogProbs> {
         const auto how = ctx->saved_data["how"].toIntVector();
         const int64_t T = tours.size(0), n = tours.size(1) - 1;
         Tensor grad = at::empty(logits.sizes(), logits.options());
-        if (n == 1) return {once(grad.zero_(), grads), Tensor(), Tensor(), Tensor()};
+        if (n == 1) return {once(grad.zero_(), grads), Tensor(), Tensor(), Tensor(), Tensor()};
         const Tensor g = grads[0].to(at::kFloat).contiguous();
         checked(api.logp_grad(ptr(logits), ptr<int64_t>(tours), ptr(state), state.numel(), ptr<float>(g), ptr(grad), T,
                               (int)n, (int)how[0], (int)how[1], logits.stride(0), logits.stride(1), code_of(logits),
                               logits.get_device(), stream_of(logits)),
                 "tsp2opt_tour_logprobs_grad");
-        return {once(grad, grads), Tensor(), Tensor(), Tensor()};
+        return {once(grad, grads), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -227,7 +229,13 @@ PYBIND11_MODULE(_learning_ext, m)
         next(api.pref_bytes); next(api.pref); next(api.pref_grad);
     });
     m.def("tour_log_probs", [](const Tensor& logits, const Tensor& tours, int64_t per, int64_t rows) {
-        return LogProbs::apply(logits, tours.to(at::kLong).contiguous(), per, rows);
+        // the library takes 32-bit sizes: what does not fit is refused here, before a copy of such arrays is made
+        constexpr int64_t most = std::numeric_limits<int32_t>::max();
+        const int64_t n = std::min(tours.size(1) - 1, most);
+        per = std::min(per, most);
+        const int64_t bytes = checked(api.logp_bytes(tours.size(0), (int)n, (int)per, (int)rows),
+                                      "tsp2opt_tour_logprobs_state_bytes");
+        return LogProbs::apply(logits, tours.to(at::kLong).contiguous(), per, rows, bytes);
     });
     m.def("policy_loss", [](const Tensor& lp, const Tensor& old, const Maybe& ref, const Tensor& adv,
                             const Maybe& mask, bool of_tour, bool of_tours, double low, double high,

@@ -285,6 +285,16 @@ def test_errors_of_the_library_keep_their_code():
     assert e.value.code == _lib.E_ARG
 
 
+def test_sizes_beyond_32_bits_are_refused_before_anything_is_copied():
+    """2^32 + 2 nodes are 2 in 32 bits; tours that share one element stand for such an array."""
+    from ml4tspbench_amd import _lib
+    ext, one = _lib.learning_ext(), torch.zeros((1, 1), dtype=torch.int64)
+    for nodes in (1 << 16, (1 << 31) + 5, (1 << 32) + 2):
+        with pytest.raises(_lib.Tsp2optError, match="65535") as e:
+            ext.tour_log_probs(torch.zeros(1, 2, 2), one.expand(1, nodes + 1), 1, 0)
+        assert e.value.code == _lib.E_UNSUPPORTED
+
+
 def test_reference_gradient_matches_differences():
     """The formula the kernels are held to, against central differences in 64 bits."""
     gen = torch.Generator().manual_seed(3)
