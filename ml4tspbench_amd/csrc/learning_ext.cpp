@@ -209,6 +209,9 @@ struct PreferenceLoss : public Function<PreferenceLoss> {
     }
 };
 
+// The library takes 32-bit sizes.  What divides an empty batch may be larger without meaning more.
+constexpr int64_t most = std::numeric_limits<int32_t>::max();
+
 // constants of a loss: never differentiated, and in the layout that the kernels read
 Tensor constant(const Tensor& x) { return x.detach().contiguous(); }
 
@@ -229,8 +232,7 @@ PYBIND11_MODULE(_learning_ext, m)
         next(api.pref_bytes); next(api.pref); next(api.pref_grad);
     });
     m.def("tour_log_probs", [](const Tensor& logits, const Tensor& tours, int64_t per, int64_t rows) {
-        // the library takes 32-bit sizes: what does not fit is refused here, before a copy of such arrays is made
-        constexpr int64_t most = std::numeric_limits<int32_t>::max();
+        // what does not fit is refused here, before a copy of such arrays is made
         const int64_t n = std::min(tours.size(1) - 1, most);
         per = std::min(per, most);
         const int64_t bytes = checked(api.logp_bytes(tours.size(0), (int)n, (int)per, (int)rows),
@@ -248,7 +250,7 @@ PYBIND11_MODULE(_learning_ext, m)
                                 const Maybe& mask, int64_t per, bool best, bool per_step, double beta,
                                 double smoothing) {
         auto out = PreferenceLoss::apply(lp, constant(ref), constant(lengths.detach().to(at::kDouble)),
-                                         constant(mask), per, (int64_t)best, (int64_t)per_step, beta, smoothing);
+                                         constant(mask), std::min(per, most), (int64_t)best, (int64_t)per_step, beta, smoothing);
         return std::make_tuple(out[0], out[1]);
     });
 }

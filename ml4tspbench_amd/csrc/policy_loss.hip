@@ -597,8 +597,9 @@ extern "C" int tsp2opt_preference_loss(const void* logp, const void* ref_logp, c
     p.per = tours_per_instance; p.best = best_only; p.per_step = per_step; p.beta = beta; p.eps = (float)label_smoothing;
     p.loss = loss_out; p.pairs = pairs_out;
     pref_state(p, state);
-    // one workgroup does all: it has 8 threads a tour, so the pairs of 512 tours take four turns of it
-    if (num_tours * steps <= kOneBlock && num_tours <= 512 && tours_per_instance <= 64) {
+    // one workgroup does all: it has 8 threads a tour, so the pairs of 512 tours take four turns of it.  No tours at all
+    // are its too, whatever an instance would have of them: the other launches would have no workgroup
+    if (num_tours == 0 || (num_tours * steps <= kOneBlock && num_tours <= 512 && tours_per_instance <= 64)) {
         const Shape s = shape_of(num_tours, steps, true);
         T2O_BY_DTYPE(dtype, T2O_BY_GROUP(s.group, hipLaunchKernelGGL((k_pref_one<E, G>), dim3(1), dim3(kOneThreads), 0,
                                                                      stream, p)));

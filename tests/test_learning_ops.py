@@ -668,6 +668,19 @@ def test_gpu_preference_loss_edges():
         assert torch.autograd.grad(res.loss, x)[0].shape == shape
 
 
+@gpu
+@pytest.mark.parametrize("pairs", ["all", "best"])
+@pytest.mark.parametrize("per", [1, 64, 65, 100, 1 << 33])
+def test_gpu_preference_loss_of_no_tours(per, pairs):
+    """An empty batch has no pair, however many tours an instance would have."""
+    import ml4tspbench_amd as amd
+    for steps in (0, 3, 20000):
+        x = torch.zeros((0, steps), device="cuda", requires_grad=True)
+        res = amd.preference_loss(x, torch.zeros(0, device="cuda"), tours_per_instance=per, pairs=pairs)
+        assert float(res.loss.detach()) == 0.0 and int(res.num_pairs) == 0
+        assert torch.autograd.grad(res.loss, x)[0].shape == x.shape
+
+
 # ------------------------------------------------------------------------------------------ GPU: streams, graphs, runs
 def whole_step(heat, tours, old, adv, length, per):
     """One training step's worth of calls: value, both losses, the heat maps' gradient."""
