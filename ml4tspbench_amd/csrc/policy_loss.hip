@@ -490,6 +490,7 @@ int policy_fill(PolicyParams& p, const void* lp, const void* old, const void* re
     if (off(state, 256)) return fail(TSP2OPT_E_ARG, "state must be 256-byte aligned");
     if (state_bytes < policy_state_bytes(T)) return fail(TSP2OPT_E_WORKSPACE, "state_bytes too small");
     if (T * S > 0 && (!lp || !old || !adv)) return fail(TSP2OPT_E_ARG, "null pointer");
+    if (T > 0 && !adv_per_step && !adv) return fail(TSP2OPT_E_ARG, "null pointer");      // read without steps too
     const size_t size = element_size(dtype);
     if (off(lp, size) || off(old, size) || off(ref, size) || off(adv, 4))
         return fail(TSP2OPT_E_ARG, "misaligned pointer (arrays must be aligned to their element size)");

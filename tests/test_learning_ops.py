@@ -273,6 +273,21 @@ def test_c_abi_checks_without_gpu():
     assert L.tsp2opt_preference_loss_grad(None, at, 8, at, at, 4, 6, 0, 0, None) == -3
 
 
+def test_c_abi_wants_advantages_of_tours_without_steps():
+    """One advantage a tour is read for every tour, also where no tour has a step."""
+    from ml4tspbench_amd import _lib
+    L, at = _lib.lib(), ctypes.c_void_p(256)
+
+    def policy(adv, T, S, per_step=0, ratio=0, average=0):
+        return L.tsp2opt_policy_loss(at, at, None, adv, None, at, at, at, 1 << 30, T, S, per_step, ratio, average, 0.2, 0.2,
+                                     0.0, 0, 0, None)
+
+    for ratio, average in ((0, 0), (0, 1), (1, 1)):
+        assert policy(None, 4, 0, 0, ratio, average) == -1 and b"null pointer" in L.tsp2opt_last_error()
+        assert policy(None, 4, 6, 0, ratio, average) == -1
+    assert policy(None, 4, 6, 1) == -1
+
+
 def test_errors_of_the_library_keep_their_code():
     """Tsp2optError.code is the library's return code, as for the operators that call it through _lib.check()."""
     from ml4tspbench_amd import _lib
