@@ -529,7 +529,7 @@ __device__ __forceinline__ void stage_tours(const LogpParams& p, Q* tile, uint16
 #pragma unroll
         for (int c = 0; c < steps; ++c) {
             const int s = min(c * 64 + lane, p.n - 1);
-            const int64_t j = t[s], i = t[s + 1];
+            const int64_t j = t[s], i = t[min(s + 1, p.n - 1)];         // nothing is chosen after the last node
             node[c] = j >= 0 && j < p.n ? (int)j : -1;
             then[c] = (int)i;
         }

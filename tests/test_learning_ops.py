@@ -401,6 +401,19 @@ def test_gpu_log_probs_pass_on_open_nan_and_inf(value):
 
 
 @gpu
+@pytest.mark.parametrize("rows,per,n", [("node", 1, 40), ("node", 3, 40), ("node", 3, 256), ("node", 3, 300), ("step", 1, 40),
+                                        ("node", 2, 1100)])
+def test_gpu_log_probs_do_not_depend_on_the_closing_entry(rows, per, n):
+    gen = torch.Generator().manual_seed(n)
+    tours = make_tours(gen, 2 * per, n)
+    logits = rows_of(gen, 2 if rows == "node" else 2 * per, n if rows == "node" else n - 1, n, torch.float32)
+    want = check_log_probs(logits, tours, per, rows, torch.Generator().manual_seed(1))
+    tours[:, n] = torch.tensor([1 << 40, -1, n, 7])[torch.arange(2 * per) % 4]
+    got = check_log_probs(logits, tours, per, rows, torch.Generator().manual_seed(1))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
 @pytest.mark.parametrize("rows", ["node", "step"])
 def test_gpu_log_probs_of_broken_tours(rows):
     """A tour with an index out of range or a repeated node gets NaN and leaves the gradient alone."""
