@@ -365,6 +365,56 @@ def test_gpu_log_probs_of_masked_and_wide_rows(n, kind, per, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=["f32", "bf16"])
+@pytest.mark.parametrize("layout,per,n,levels", [                       # spread: one column in seven is high
+    ("spread", 2, 15, (0, -90)), ("spread", 18, 140, (0, -90)), ("spread", 3, 140, (0, -35, -90)),
+    ("spread", 2, 270, (0, -90)), ("spread", 17, 270, (0, -90)), ("spread", 2, 1030, (0, -90)), ("spread", 2, 2070, (0, -90)),
+    ("parts", 1, 1030, (0, -90)), ("parts", 1, 1030, (0, -35)), ("parts", 2, 1030, (0, -35)), ("parts", 2, 1030, (0, -60)),
+    ("parts", 1, 2070, (0, -35, -90)), ("parts", 2, 2070, (0, -35, -60)), ("parts", 2, 2070, (0, -60, -90)),
+    ("parts", 2, 2070, (-60, 0, -90)), ("parts", 2, 3100, (0, -60, -90, -35))])
+def test_gpu_log_probs_of_steps_whose_sum_is_tiny(layout, per, n, levels, dtype):
+    """Steps whose open entries lie 35 .. 90 below their row's maximum and still are in its sum, which then is around
+    2^-50 .. 2^-130: what long tours end with where a map is sure of its first edges.  The high nodes are visited
+    first.  With the levels in blocks of columns every part of a long row has a maximum of its own, far from the
+    others'.  The tolerance is the formula's: exponentials at a distance of 100 carry 100 u of the difference and 100 u
+    of the argument, the logarithm of such a sum and the difference that is left round 100 u each, below the 8 u (64 + 90)
+    that it allows for.  A tour's term g p of the gradient, p = exp(h - m) / S with S >= 1, is lost where the hardware's
+    exponential is below 2^-126, the smallest number that it gives (e^-90 is 2^-130): off by |g| 2^-126 a tour."""
+    import ml4tspbench_amd as amd
+    gen = torch.Generator().manual_seed(n + per)
+    j = torch.arange(n)
+    parts = (n + 1023) // 1024
+    width = (-(-n // parts) + 63) // 64                     # entries a lane, in the steps of 12 and 16 that these sizes take
+    width = 64 * (12 if width <= 12 else 16)
+    level = torch.tensor(levels, dtype=torch.float32)
+    which = (j // width).clamp(max=len(levels) - 1) if layout == "parts" else torch.where(j % 7 == 0, 0, 1 + j % (len(levels) - 1))
+    logits = (torch.randn((1, n, n), generator=gen) + level[which]).to(dtype)
+    tours = torch.zeros((per, n + 1), dtype=torch.int64)
+    for k in range(per):
+        noise = torch.rand(n, generator=gen)
+        tours[k, :n] = (-level[which] + 0.5 * noise).argsort()
+        tours[k, n] = tours[k, 0]
+    # such sums are there: base two, relative to the row's maximum without its diagonal
+    x = logits[0][tours[0, :-2]].double()
+    x[torch.arange(n - 1), tours[0, :-2]] = -math.inf
+    top = x.amax(1, keepdim=True)
+    seen = (x - top).gather(1, tours[0, None, :n].expand(n - 1, n)).masked_fill_(torch.ones((n - 1, n), dtype=torch.bool).tril(), -math.inf)
+    size = seen.logsumexp(1) / math.log(2)
+    deep = min(levels)
+    assert int(((size < (deep + 6) / math.log(2)) & (size > -139)).sum()) >= 3
+    if deep == -90:
+        assert int(((size < -121) & (size > -139)).sum()) >= 3
+    g = torch.randn((per, n - 1), generator=gen)
+    g[torch.rand(g.shape, generator=gen) < 0.1] = 0.0
+    lp, tol, grad, gtol = ref_log_probs(logits, tours, per, "node", g)
+    heat = logits.cuda().requires_grad_()
+    got = amd.tour_log_probs(heat, tours.cuda(), tours_per_map=per)
+    (dx,) = torch.autograd.grad(got, heat, g.cuda())
+    compare("log-probabilities", got, lp, tol)
+    compare("gradient", dx, grad, gtol + per * float(g.abs().max()) * 2.0 ** -126)
+
+
+@gpu
 @pytest.mark.parametrize("per", [1, 3])
 @pytest.mark.parametrize("n", [6, 70, 300, 1031, 2060])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf, 3.0e38])
