@@ -6,8 +6,8 @@ an autoregressive decoder wrote), with gradients for ``torch.autograd``: ``tour_
 ``clipped_policy_loss`` and ``preference_loss`` (csrc/policy_loss.hip).
 
 Everything runs on the current stream of the tensors' device, without host synchronisation, and may be captured into a
-graph; results do not change from run to run.  There is no CPU path, and no second derivative.  The autograd nodes are
-csrc/learning_ext.cpp.
+graph; results do not change from run to run.  There is no CPU path, no second derivative, no ``torch.func`` transform
+and no forward mode: all of them raise.  The autograd nodes are csrc/learning_ext.cpp.
 """
 from __future__ import annotations
 

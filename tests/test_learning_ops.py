@@ -924,6 +924,34 @@ def test_gpu_refusals_of_the_library_keep_their_code():
 
 
 @gpu
+@pytest.mark.parametrize("op", ["log_probs", "policy", "preference"])
+def test_gpu_function_transforms_and_forward_mode_raise(op):
+    """vmap, torch.func.grad and forward-mode derivatives are not offered: they raise instead of giving something else."""
+    import ml4tspbench_amd as amd
+    heat, tours, old, adv, length, per = step_inputs(8, M=2, per=2, n=20)
+    x = heat if op == "log_probs" else old.detach()
+
+    def value(x):
+        if op == "policy":
+            return amd.clipped_policy_loss(x, old, adv).loss
+        if op == "preference":
+            return amd.preference_loss(x, length, tours_per_instance=per).loss
+        return amd.tour_log_probs(x, tours, tours_per_map=per).sum()
+
+    value(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(value)(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(value)(torch.stack([x, x]))
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(value, (x,), (torch.ones_like(x),))
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        value(fwd.make_dual(x, torch.ones_like(x)))
+    value(x)
+
+
+@gpu
 def test_gpu_run_of_decoder_two_opt_evaluation_and_losses():
     """As they are used: tours of heat maps are scored, improved, measured, and the losses' gradient comes back to the
     maps; every value against the formulas, chained in 64 bits on the CPU."""
