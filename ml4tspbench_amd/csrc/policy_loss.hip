@@ -64,6 +64,13 @@ __device__ __forceinline__ bool is_cut(const PolicyParams& p, float adv, double 
     return (adv > 0.0f && x > p.log_hi) || (adv < 0.0f && x < p.log_lo);
 }
 
+// -adv e^x where it is not cut.  An advantage of 0 makes it 0 also where e^x is past the range of float, which would give
+// 0 times inf; the steps of a long tour sum up to such an x.
+__device__ __forceinline__ float ratio_term(float adv, double x)
+{
+    return adv == 0.0f && x < __builtin_inf() ? 0.0f : -adv * expf((float)x);
+}
+
 // Sum over a group of G threads (over the workgroup where G is more than a wave), in every thread of it.
 template <int G, int N>
 __device__ __forceinline__ void group_sum(double (&v)[N])
@@ -171,7 +178,7 @@ __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
                     v[4] += x;
                 } else {
                     const bool cut = is_cut(p, adv[u], x);
-                    v[0] += (double)(-adv[u] * (cut ? (adv[u] > 0.0f ? p.hi : p.lo) : expf((float)x)));
+                    v[0] += (double)(cut ? -adv[u] * (adv[u] > 0.0f ? p.hi : p.lo) : ratio_term(adv[u], x));
                     v[2] += cut ? 1.0 : 0.0;
                 }
                 if (p.ref) v[1] += (double)kl_term(ref[u] - lp[u]);
@@ -188,7 +195,7 @@ __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
         if (p.mode & kRatioTour) {
             const float adv = p.adv[k];
             const bool cut = is_cut(p, adv, v[4]);
-            c = cut ? 0.0f : -adv * expf((float)v[4]);
+            c = cut ? 0.0f : ratio_term(adv, v[4]);
             v[0] = cut ? -adv * (adv > 0.0f ? p.hi : p.lo) : c;
             v[2] = cut ? 1.0 : 0.0;
         } else {
@@ -243,7 +250,7 @@ __global__ __launch_bounds__(1024) void k_policy_grad(PolicyParams p)
                         d = row.x;
                     } else {
                         const double x = (double)lp[u] - (double)old[u];
-                        d = is_cut(p, adv[u], x) ? 0.0f : -adv[u] * expf((float)x) * row.y;
+                        d = is_cut(p, adv[u], x) ? 0.0f : ratio_term(adv[u], x) * row.y;
                     }
                     if (p.ref && p.kl_coef != 0.0) {
                         const float e = ref[u] - lp[u];

@@ -664,6 +664,35 @@ def test_gpu_policy_loss_edges():
 
 
 @gpu
+@pytest.mark.parametrize("ratio,average,per_step", [("step", "step", False), ("step", "step", True), ("step", "tour", False),
+                                                    ("tour", "tour", False)])
+def test_gpu_policy_loss_of_zero_advantages_and_far_ratios(ratio, average, per_step):
+    """A tour of advantage 0 (an instance whose tours are equally long) adds nothing, however far its ratio has gone:
+    e^100 is past the range of float, its product with 0 is 0."""
+    import ml4tspbench_amd as amd
+    gen = torch.Generator().manual_seed(17)
+    T, S = 6, 50
+    old = -torch.rand((T, S), generator=gen) - 0.5
+    lp = old + 0.02 * torch.randn((T, S), generator=gen)
+    adv = torch.randn(T, generator=gen)
+    old[1, 7] -= 100.0
+    old[2] -= 2.5                       # 125 for the tour
+    old[3, 0] = -math.inf               # e^inf is no number that 0 would win over: masked
+    adv[1:4] = 0.0
+    mask = torch.ones((T, S), dtype=torch.bool)
+    mask[3, 0] = False
+    if per_step:
+        adv = adv[:, None].expand(T, S).contiguous()
+    check_policy(lp, old, None, adv, mask, ratio, average, 0.0)
+    x = lp.cuda().requires_grad_()
+    res = amd.clipped_policy_loss(x, old.cuda(), torch.zeros_like(adv).cuda(), mask=mask.cuda(), ratio=ratio, average=average)
+    assert float(res.loss.detach()) == 0.0 and float(res.clip_fraction) == 0.0
+    assert not torch.autograd.grad(res.loss, x)[0].any()
+    lost = amd.clipped_policy_loss(x, old.cuda(), adv.cuda(), ratio=ratio, average=average)      # and unmasked it is NaN
+    assert math.isnan(float(lost.loss.detach()))
+
+
+@gpu
 def test_gpu_policy_loss_small_kl_keeps_its_digits():
     """d of 1e-4: exp(d) - 1 - d is 5e-9, of which float32 subtraction would leave nothing."""
     import ml4tspbench_amd as amd
