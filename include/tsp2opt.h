@@ -259,8 +259,8 @@ int tsp2opt_gls_rounds(const double* points, int64_t* tours, int64_t* best_tours
  * Learning operators: from tours back to the heat map (or the autoregressive decoder) they were drawn from.
  * No counterpart in the reference's native code; its trainers do this with chains of torch kernels per decoding step.
  * All of them only enqueue kernels on `hip_stream` (no allocation, no memset, no host synchronisation; they may be
- * captured), use no atomics, add in a fixed order (bit-identical from run to run) and compute in float with double
- * sums over steps; `dtype` (TSP2OPT_DTYPE_F32, _BF16 or _F16) is only how an array is stored.  `state` is device memory
+ * captured), use no atomics whose order could matter, add in a fixed order (bit-identical from run to run) and compute
+ * in float with double sums over steps; `dtype` (TSP2OPT_DTYPE_F32, _BF16 or _F16) is only how an array is stored.  `state` is device memory
  * of the caller, 256-byte aligned, written by the forward call and read by its gradient call.
  *
  * tsp2opt_tour_logprobs -- step log-probabilities of tours (sampling procedure ml4tsp/nar/decoder/sampling.py:21-43 on

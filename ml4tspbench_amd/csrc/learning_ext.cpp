@@ -2,8 +2,8 @@
 //
 // The forward and gradient entry points of libtsp2opt_hip.so as torch::autograd nodes.  Written in C++ because the
 // losses are a few microseconds of GPU work: a node in Python has autograd's device thread wait for the interpreter
-// lock on every backward pass (clipped_policy_loss on 16 x 49 steps, forward and gradient: 129 us through Python
-// nodes, 38..60 us through these).  The entry points are handed over by ml4tspbench_amd/learning.py, so
+// lock on every backward pass (clipped_policy_loss on 16 x 49 steps, forward and gradient: 127 us through Python
+// nodes, 58 us through these).  The entry points are handed over by ml4tspbench_amd/learning.py, so
 // that there is one copy of the library in the process, the one that _lib.py loaded.
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>

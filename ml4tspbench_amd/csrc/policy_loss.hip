@@ -5,7 +5,9 @@
 // Preference loss over pairs (a, b) of one instance's tours, a the shorter, with s = beta sum(lp - ref):
 //     l = -(1 - eps) log sigmoid(s_a - s_b) - eps log sigmoid(s_b - s_a)
 // Both are averages; the gradients are recomputed from the same inputs in one pass.  Sums over steps and rows are
-// kept in double and added in a fixed order: results do not depend on the schedule.
+// kept in double and added in a fixed order: results do not depend on the schedule.  What is summed is a float: a step's
+// or a pair's term carries a few 2^-24 of itself (a score difference z is rounded to float, and its sigmoid is off by
+// |z| 2^-24 of itself for it), the precision that loss and gradient are given in.
 //
 // A row of steps is read by a group of G threads: 8 or 16 for short rows, a wave, or for long rows of few tours a whole
 // workgroup.  Bound by memory where there is much (10000 x 1000 steps in float32 with reference and mask: 130 MB read in

@@ -22,7 +22,10 @@
 // That sum loses steps whose open entries all lie far below the row's maximum, so the exponentials are kept times 2^60,
 // which spends the range of float above 1 too: what it flushes (below 2^-126, 65535 entries at most) is under 2^-30 of a
 // sum above 2^-80, which is 2^-140 = e^-97 relative to the row's maximum.  Steps below that (and those that are NaN) are
-// redone alone, relative to their own maximum.
+// redone alone, relative to their own maximum.  The others are rounded at their distance from the row's maximum and not
+// from their own: 2^-24 of up to 97, the price of one exponential for all tours.  On 16 TSP-500 maps exp(-distance / tau)
+// with 256 sampled tours the largest error of a log-probability is 7.6e-6 and their root mean square 1.9e-7; with every
+// step's own maximum (k_single) 9.7e-7 and 8.6e-8.
 // One tour a row (k_single): the maximum is the open entries' own, nothing is ever lost.
 #include "learn_common.hpp"
 
@@ -593,7 +596,8 @@ struct SharedWork {
 };
 
 // Reads the rows once and adds kRows rows up for a tour with every position that it reads from LDS.  128 maps x 16 tours of
-// 500 nodes: 60 us in float32, 50 us in bfloat16.  Of the 60, reading and exponentiating the rows alone takes 32 us
+// 500 nodes: 60 us in float32, 50 us in bfloat16 under the profiler, where every launch ends by itself (in a stream of
+// passes 57 and 49 us, the 7 us of k_positions included).  Of the 60, reading and exponentiating the rows alone takes 32 us
 // (128 MB, the rate of any large read here), the masked additions 22 and the ends of the steps 6: the workgroups of a unit
 // run their phases side by side and overlap little.  Measured and left out: 6 instead of 4 waves a SIMD by limiting the
 // registers (the same), workgroups of four waves (53 and 65 us), several blocks of rows in a workgroup with the next one's

@@ -17,8 +17,9 @@
 // adjacent diagonals as two "streams" A and B of 4 and walks rows in macro steps of 4 (32 pairs,
 // 32 sqrt); two macro steps make a TILE of 8 rows x 8 diagonals.  Every value of a step is an
 // (A, B) register pair; the build keeps the compiler from packing them (v_pk_add/mul/fma_f32 would take 25
-// SIMD-cycles per 64 pairs against 37 for the scalar form, tools/valu_chain_microbench.hip, but have given
-// wrong results now and then), which costs the TSP-500 x 2048 batch 15.1 -> 17.4 ms.  Tour-ordered, centred and scaled fp32 coordinates sit in LDS as
+// SIMD-cycles per 64 pairs against 37 for the scalar form, tools/valu_chain_microbench.hip; build.py says why
+// they are kept out), which costs the TSP-500 x 2048 batch 15.1 -> 17.4 ms.  Tour-ordered, centred and scaled
+// fp32 coordinates sit in LDS as
 // three 8-way interleaved arrays (x, y, edge length) whose entries are already the (A, B) pairs
 // (value at window position w and at w + 4), so one conflict-free ds_read_b64 per operand feeds the
 // math with no register moves; row operands are broadcast reads of the same arrays.
