@@ -13,7 +13,7 @@ distributed, RCCL), every rank solves its own batch of the same shape (weak scal
 collective) and the timed region ends with one all_gather of tours + lengths.
 
 metric: pair-deltas/s = sum over tours of sweeps * (N-1)(N-2)/2 / wall time, sweeps = iterator+1
-when converged else the cap (SURVEY.md 8d).  Prints ONE JSON line on rank 0.
+when converged else the cap.  Prints ONE JSON line on rank 0.
 
 The default invocation (no --config) times the headline exactly as above (W warm-up steps, K timed
 steps, top-level keys) and then, outside that timed region, adds to the SAME line:
@@ -48,9 +48,9 @@ CONFIGS = {
     "tsp1000": (1000, 128, 1),
     "tsp10000": (10000, 16, 1),
 }
-FLOP_PER_PAIR = 15.0          # SURVEY.md 8(d3): 2 x (2 sub + 2 mul + add + sqrt) + 3 add/sub
-PEAK_FP32_VALU_TFLOPS = 157.3  # MI355X_MICROARCH.md: 256 CU x 2.4 GHz x 256 FLOP/clk/CU
-PEAK_FP64_VALU_TFLOPS = 78.6   # SURVEY.md 8(d3) / BASELINE.md: the fp64 vector peak
+FLOP_PER_PAIR = 15.0          # 2 x (2 sub + 2 mul + add + sqrt) + 3 add/sub
+PEAK_FP32_VALU_TFLOPS = 157.3  # 256 CU x 2.4 GHz x 256 FLOP/clk/CU
+PEAK_FP64_VALU_TFLOPS = 78.6   # the fp64 vector peak
 # tools/valu_chain_microbench.hip: SIMD cycles per 64 evaluated pairs of the scalar
 # per-pair chain (1 v_sqrt_f32, sub / mul / fma / add, min) -- the instruction floor of the sweep; the build uses no
 # packed FP32 instructions
@@ -181,7 +181,7 @@ def cpu_baseline(name: str, pts: np.ndarray, tours: np.ndarray, tpi: int, group:
     """The oracle (oracle/two_opt_oracle.c, a port of the reference algorithm) timed on this box's
     host cores on a bounded sample of the same workload (about 20 s of CPU work): the first `want`
     tours, and for sizes where even one tour per core exceeds the budget (TSP-10000) also a lower
-    iteration cap.  BASELINE.md 2 / SURVEY 8 d4 ask for two legs: OpenMP over tours on the box's cores
+    iteration cap.  Two legs: OpenMP over tours on the box's cores
     (the dict itself) and one core (`single_core`, about 2 s of the same sample).
     Returns the baseline dict, the oracle's tours/iterations and the cap it ran with."""
     from oracle import two_opt_oracle as orc
@@ -230,9 +230,9 @@ def cpu_baseline(name: str, pts: np.ndarray, tours: np.ndarray, tpi: int, group:
 
 
 def dense_torch_baseline(pts: np.ndarray, tours: np.ndarray, tpi: int, budget_s: float = 4.0):
-    """The reference's COST STRUCTURE on the host (SURVEY.md 8d4, reported baseline only): a dense
+    """The reference's COST STRUCTURE on the host (reported baseline only): a dense
     torch formulation of the same best-improvement step -- all N x N deltas of a (P, N+1) batch as
-    tensors, argmin, host read-back, reversal -- written from the algorithm's definition (SURVEY 3.4),
+    tensors, argmin, host read-back, reversal -- written from the algorithm's definition,
     fp64, torch CPU threads.  Timed per iteration on the first instance's tours for a bounded time."""
     n = pts.shape[1]
     P = torch.from_numpy(pts[0])
@@ -582,8 +582,9 @@ def main():
                             "frac_fp64_peak and may exceed 1.  The kernel re-evaluates only pairs_evaluated_frac of the "
                             "pairs per sweep (tile-minimum cache, reversals folded onto the shorter side of the cycle) "
                             "at one distance per pair: executed_*, insn_floor_frac and valu_busy are what the VALUs "
-                            "really did (rocprofv3 PMC passes of this build; a packed instruction counts once, so "
-                            "executed_tflops is a lower bound).  HBM traffic is O(N) per tour."}
+                            "really did (rocprofv3 PMC passes of this build; executed_tflops counts fused "
+                            "multiply-adds twice, additions, products and square roots once, and no minima).  "
+                            "HBM traffic is O(N) per tour."}
         if strong:
             work = (f"TSP-{n} uniform, ONE batch of {inst} instances x {tpi} random start tours sharded over "
                     f"{world} GPU(s) by sharding.solve_sharded (contiguous instance blocks)")

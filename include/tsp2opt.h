@@ -85,7 +85,7 @@ extern "C" {
  *            call is asynchronous with respect to the host
  *
  * Results: bit-identical tours to the reference algorithm evaluated with IEEE-754 correctly
- * rounded +,-,*,sqrt in `dtype` and first-flat-index argmin tie-breaking (see DESIGN.md).
+ * rounded +,-,*,sqrt in `dtype` and first-flat-index argmin tie-breaking.
  */
 int tsp2opt_solve(const void* points, int64_t* tours, int32_t* iters_out, int32_t* sweeps_out,
                   double* lengths_out, int32_t* status_out, int64_t num_tours, int32_t n,
@@ -334,13 +334,13 @@ int tsp2opt_preference_loss_grad(const uint8_t* mask, const void* state, int64_t
 /*
  * tsp2opt_sqrt_check -- numerics self-test used by the GPU test-suite: out[k] = sqrt(in[k])
  * computed with the exact device routine the delta evaluation uses (dtype as above).  Lets the
- * tests prove 0-ulp agreement with the host's correctly rounded sqrt (SURVEY.md hard part b).
+ * tests prove 0-ulp agreement with the host's correctly rounded sqrt.
  */
 int tsp2opt_sqrt_check(const void* in, void* out, int64_t count, int32_t dtype, int32_t device,
                        void* hip_stream);
 
 /* Kernel variant / launch geometry the library would pick for n (for logs and tests): the geometry of batches with
- * more tours than compute units (smaller batches get two to four times the threads per tour, DESIGN.md 4.1b).
+ * more tours than compute units (smaller batches get two to four times the threads per tour).
  * out[0]=threads per workgroup, out[1]=fast-path class (0: exact-only kernel), out[2]=LDS bytes,
  * out[3]=row segments, out[4]=diagonal groups, out[5]=macro steps, out[6]=resident workgroups/CU */
 int tsp2opt_plan(int32_t n, int32_t dtype, int32_t device, int32_t* out7);

@@ -1,4 +1,4 @@
-// ml4tspbench_amd/csrc/greedy.hip -- greedy edge-merge decoder on gfx950 (SURVEY.md 8f row f1)
+// ml4tspbench_amd/csrc/greedy.hip -- greedy edge-merge decoder on gfx950
 //
 // Replaces (reference, read-only): search/greedy_search.py:19-74 (tsp_greedy) and
 // search/cython_merge/sources/cython_merge.pyx:19-120 (merge_cython): symmetrise the heat map,

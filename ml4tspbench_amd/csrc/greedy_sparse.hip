@@ -1,4 +1,4 @@
-// ml4tspbench_amd/csrc/greedy_sparse.hip -- greedy edge-merge decoder for SPARSE heat maps (SURVEY.md 8f row f1)
+// ml4tspbench_amd/csrc/greedy_sparse.hip -- greedy edge-merge decoder for SPARSE heat maps
 //
 // Replaces (reference, read-only) the sparse branch of tsp_greedy (search/greedy_search.py:39-47) +
 // merge_cython (search/cython_merge/sources/cython_merge.pyx:19-120): the reference densifies the

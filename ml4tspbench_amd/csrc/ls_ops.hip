@@ -1,4 +1,4 @@
-// ml4tspbench_amd/csrc/ls_ops.hip -- the reference's other move operators on gfx950 (SURVEY.md 8f row f4)
+// ml4tspbench_amd/csrc/ls_ops.hip -- the reference's other move operators on gfx950
 //
 // Replaces (reference, read-only): get_two_opt_tour / get_relocate_tour and their helpers
 // (search/local_search.py:9-105, search/relocate.py:5-38; the same functions again in

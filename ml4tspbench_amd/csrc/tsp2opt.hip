@@ -3,7 +3,7 @@
 // Batched best-improvement 2-opt local search, the whole improvement loop on the device.
 // Replaces (reference, read-only): search/two_opt.py:21-48 and
 // ml4tsp-library/ml4tsp/nar/local_search/two_opt.py:34-65 (+ the per-tour Python loop of
-// ml4tsp-library/ml4tsp/nar/local_search/base.py:58-64).  Design: DESIGN.md.
+// ml4tsp-library/ml4tsp/nar/local_search/base.py:58-64).
 //
 // One workgroup owns one tour.  Per iteration it must find the reference's argmin over all
 // position pairs (i, j >= i+2) of
@@ -88,7 +88,7 @@ struct ProfSlot {
 // Test / diagnostic knobs (tsp2opt_debug_*, tsp2opt_profile_enable).  They belong to the CALLING THREAD:
 // a setter changes the calling thread's copy, and every entry point snapshots its own thread's copy once
 // on entry, so a knob flipped by one thread never changes a call running on another (one thread per
-// device is the supported concurrency, INTEGRATION.md).
+// device is the supported concurrency).
 struct Opts {
     int profile = 0;            // HIP events around the persistent kernel (tsp2opt_profile_enable)
     int dbg_sweeps = 0;         // filter sweeps only (tsp2opt_debug_sweep_only)

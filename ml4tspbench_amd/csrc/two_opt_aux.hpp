@@ -1,5 +1,5 @@
 // ml4tspbench_amd/csrc/two_opt_aux.hpp -- coupled-mode glue, tour lengths, validation/evaluation and numerics self-test kernels
-// Part of the single translation unit tsp2opt.hip (design notes at its top and in DESIGN.md).
+// Part of the single translation unit tsp2opt.hip (design notes at its top).
 #pragma once
 
 namespace t2o {

@@ -1,5 +1,5 @@
 // ml4tspbench_amd/csrc/two_opt_band.hpp -- band cluster kernel k_two_opt_cluster (several workgroups per tour, N beyond the fast path)
-// Part of the single translation unit tsp2opt.hip (design notes at its top and in DESIGN.md).
+// Part of the single translation unit tsp2opt.hip (design notes at its top).
 #pragma once
 
 namespace t2o {

@@ -1,5 +1,5 @@
 // ml4tspbench_amd/csrc/two_opt_common.hpp -- constants, parameter blocks, LDS view, exact arithmetic of the 2-opt kernels
-// Part of the single translation unit tsp2opt.hip (design notes at its top and in DESIGN.md).
+// Part of the single translation unit tsp2opt.hip (design notes at its top).
 #pragma once
 
 namespace t2o {

@@ -1,5 +1,5 @@
 // ml4tspbench_amd/csrc/two_opt_kernel.hpp -- filter sweep, incremental sweeps, argmin selection, reversal, cluster exchange, k_two_opt
-// Part of the single translation unit tsp2opt.hip (design notes at its top and in DESIGN.md).
+// Part of the single translation unit tsp2opt.hip (design notes at its top).
 #pragma once
 
 namespace t2o {

@@ -1,4 +1,4 @@
-"""Host-side mirror of the reference's greedy edge-merge decoder (SURVEY.md 8f row f1).
+"""Host-side mirror of the reference's greedy edge-merge decoder.
 
 Reference interface (read-only): ``search/greedy_search.py:19-74`` ``tsp_greedy`` (registered as
 ``DECODING_CLASS[('tsp', 'greedy')]``, ``search/__init__.py:36``) on top of the Cython

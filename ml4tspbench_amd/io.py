@@ -1,4 +1,4 @@
-"""Instance / tour text format of the reference datasets (SURVEY.md 8f row f4).
+"""Instance / tour text format of the reference datasets.
 
 One instance per line:  ``x0 y0 x1 y1 ... output t0 t1 ... t0`` with 1-based node indices
 (writer: ``generate.py:147-153``; reader/writer: ``solvers/solver.py:51-78,115-138``).  Tours come

@@ -1,4 +1,4 @@
-"""Host-side mirror of the reference's other local searches (SURVEY.md 8f row f4).
+"""Host-side mirror of the reference's other local searches.
 
 Reference interface (read-only):
   * ``search/relocate.py:40-61``      ``tsp_relocate`` -- one best relocate move per tour

@@ -1,6 +1,6 @@
 """Multi-GPU sharding of the batched 2-opt: one process per GPU, torch.distributed (RCCL on ROCm).
 
-The path shards by construction (SURVEY.md 8e): tours are independent (``group_size == 1``) or
+The path shards by construction: tours are independent (``group_size == 1``) or
 independent groups of ``P`` tours (coupled mode); an instance's tours stay on one rank so each rank
 only touches its own instances' coordinates.  There is NO per-iteration collective: every rank runs
 the persistent kernel on its block of instances, then ONE ``all_gather`` of tours, iteration counts and
@@ -8,7 +8,7 @@ lengths ends the call (TSP-500 x 2048: 8.2 MB in total).
 
 Two input forms:
   * replicated (default): every rank holds the whole batch and solves the instances ``assign_units`` gives
-    it -- contiguous blocks (default), interleaved, or balanced by a cost proxy (SURVEY 8e1: iteration
+    it -- contiguous blocks (default), interleaved, or balanced by a cost proxy (iteration
     counts vary 2-3x between greedy-start tours, and the slowest rank sets the time);
   * ``local_inputs=True``: every rank passes ONLY its own block ("each GPU gets its instances'
     coordinates only"); the whole batch is the concatenation of the blocks in rank order.

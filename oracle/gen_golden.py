@@ -8,7 +8,7 @@ The fixtures are data (inputs and expected outputs); no reference source is copi
 
     python oracle/gen_golden.py [--only G1,G3] [--skip-existing]
 
-Two runs per case (see DESIGN.md "What bit-exact means"):
+Two runs per case (bit-exact: the same tours and iteration counts):
   * "ieee":   the reference code with ``torch.sqrt`` swapped for an IEEE-754 correctly rounded
               square root (numpy's, i.e. the hardware instruction).  This is what the reference
               computes on a CUDA device (``sqrt.rn``) and on CPU builds without MKL VML, and it is
@@ -312,7 +312,7 @@ def g9(ref):   # edge cases
     pts = (centers[rng.integers(0, 5, size=(4, 120))] + 0.02 * rng.standard_normal((4, 120, 2)))
     tours = [random_tour(rng, 120) for _ in range(4)]
     case("g9_n120_clustered_f64", ref, pts, tours)
-    # int32 tours are accepted by the reference (SURVEY 8a); stored as int64 here
+    # int32 tours are accepted by the reference; stored as int64 here
     pts = uniform_points(rng, 2, 33)
     tours = [random_tour(rng, 33) for _ in range(2)]
     case("g9_n33_indep_f64", ref, pts, tours)

@@ -1,5 +1,5 @@
 """oracle/gen_golden_eval.py -- TEST INFRASTRUCTURE: makes tests/golden/eval_*.npz and
-tests/golden/txt_format_lines.txt (SURVEY.md 8f rows f2 and f4).
+tests/golden/txt_format_lines.txt.
 
 Runs ONLY in the build container, where /root/reference exists.
 

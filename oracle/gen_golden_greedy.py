@@ -1,5 +1,5 @@
 """oracle/gen_golden_greedy.py -- TEST INFRASTRUCTURE: golden vectors for the greedy edge-merge
-decoder (SURVEY.md 8f row f1).  Build container only.
+decoder.  Build container only.
 
 Runs the reference's own ``tsp_greedy`` (``search/greedy_search.py:19-74``) with its own Cython
 merge (``search/cython_merge/sources/cython_merge.pyx``, compiled by

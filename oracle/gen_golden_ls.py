@@ -1,5 +1,5 @@
-"""oracle/gen_golden_ls.py -- TEST INFRASTRUCTURE: makes tests/golden/ls_*.npz (SURVEY.md 8f row f4,
-"the other move operators").
+"""oracle/gen_golden_ls.py -- TEST INFRASTRUCTURE: makes tests/golden/ls_*.npz
+(the other move operators).
 
 Runs ONLY in the build container, where /root/reference exists.  Loads the reference's
 ``search/relocate.py`` and ``search/local_search.py`` by file path (numpy / scipy / itertools only; the

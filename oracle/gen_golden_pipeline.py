@@ -8,7 +8,7 @@ The reference chains the two steps in its test loop (``models/modelzoo/gnn/tsp_g
 call when parallel_sampling > 1.  This script does exactly that with the reference's own functions
 (``tsp_greedy`` with its Cython merge compiled into oracle/_ref/, loaded as in gen_golden_greedy.py;
 ``two_opt.py`` loaded by file path as in gen_golden.py, ``torch.sqrt`` swapped for the IEEE square root
--- DESIGN.md "What bit-exact means") and stores heat map -> decoded tours -> final tours.
+-- the same tours and iteration counts) and stores heat map -> decoded tours -> final tours.
 
 Fixtures (tests/golden/pipe_*.npz): points (N,2) f64, heatmap (P,N,N) f32 [dense] or values (P,E) +
 edge_index (2,E) [sparse], decoded (P,N+1) int64, tours_out (P,N+1) int64, iterator () int64 (ieee run),

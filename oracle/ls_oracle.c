@@ -1,7 +1,7 @@
 /*
  * oracle/ls_oracle.c -- TEST INFRASTRUCTURE, NOT PRODUCT CODE.
  *
- * Scalar CPU restatement of the reference's other move operators (SURVEY.md 8f row f4):
+ * Scalar CPU restatement of the reference's other move operators:
  *   two_opt_cost / get_two_opt_tour / swap      search/local_search.py:9-53
  *   relocate_cost / get_relocate_tour / relocate search/local_search.py:56-105, search/relocate.py:5-38
  *   local_search                                 search/local_search.py:125-134

@@ -29,7 +29,7 @@ d = {
     "sqrt_lanes (TRANS_F32 x64 = pair-deltas actually evaluated by the filter)": 64 * out.get("SQ_INSTS_VALU_TRANS_F32", 0),
     "hbm_bytes (FETCH_SIZE*2 + WRITE_SIZE) KiB->B, gfx950 read correction": (2 * out.get("FETCH_SIZE", 0) + out.get("WRITE_SIZE", 0)) * 1024,
   },
-  "note": "per launch (one k_two_opt launch per pass); a packed v_pk_* instruction is one count in the "
-          "SQ_INSTS_VALU_*_F32 counters although it produces two results, so fp32_flop_executed is a lower bound",
+  "note": "per launch (one k_two_opt launch per pass); fp32_flop_executed leaves out minima and comparisons (a build "
+          "with packed v_pk_* instructions would count each of them once although it gives two results)",
 }
 print(json.dumps(d, indent=1))
