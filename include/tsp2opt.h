@@ -260,8 +260,8 @@ int tsp2opt_gls_rounds(const double* points, int64_t* tours, int64_t* best_tours
  * No counterpart in the reference's native code; its trainers do this with chains of torch kernels per decoding step.
  * All of them only enqueue kernels on `hip_stream` (no allocation, no memset, no host synchronisation; they may be
  * captured), use no atomics whose order could matter, add in a fixed order (bit-identical from run to run) and compute
- * in float with double sums over steps; `dtype` (TSP2OPT_DTYPE_F32, _BF16 or _F16) is only how an array is stored.  `state` is device memory
- * of the caller, 256-byte aligned, written by the forward call and read by its gradient call.
+ * in float with double sums over steps; `dtype` (TSP2OPT_DTYPE_F32, _BF16 or _F16) is only how an array is stored.
+ * `state` is device memory of the caller, 256-byte aligned, written by the forward call and read by its gradient call.
  *
  * tsp2opt_tour_logprobs -- step log-probabilities of tours (sampling procedure ml4tsp/nar/decoder/sampling.py:21-43 on
  * the heat map exp(logits)): step s = 0 .. n-2 of tour t chooses t[s+1] among the nodes not visited yet with the
@@ -290,7 +290,8 @@ int tsp2opt_tour_logprobs_grad(const void* logits, const int64_t* tours, const v
 /*
  * tsp2opt_policy_loss -- clipped policy loss with a KL term on step log-probabilities (num_tours, steps):
  *   x = logp - old_logp (ratio_of_tour: summed over the tour's kept steps), r = exp x,
- *   term = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(d) - 1 - d with d = ref_logp - logp per step,
+ *   term = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), 0 for A = 0 and x < inf,
+ *   kl = exp(d) - 1 - d with d = ref_logp - logp per step,
  *   loss = average(term) + kl_coef * average(kl)
  *   average_of_tours 0: over all kept steps; 1: over a tour's kept steps, then over the tours that have any
  *   ref_logp  NULL: no KL term (kl_coef must be 0, else finite)

@@ -112,7 +112,8 @@ def clipped_policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, ad
     or with ``ratio="tour"`` of the tour's summed difference (advantages (T,)), plus ``kl_coef`` times
     ``exp(d) - 1 - d``, ``d = ref_log_probs - log_probs`` of every step.  ``average="step"`` (the default for ratios of
     steps): over all steps that count; ``"tour"`` (always for ratios of tours): over a tour's steps, then over the tours
-    that have any.  Nothing that counts: loss 0.  Steps of -inf now and then alike (forbidden edges) give NaN: mask them.
+    that have any.  Nothing that counts: loss 0; an advantage of 0 adds 0 however far its ratio has gone.  Steps of -inf
+    now and then alike (forbidden edges) give NaN: mask them.
     Asynchronous on the current stream."""
     _step_arrays(log_probs, mask, old_log_probs=old_log_probs, ref_log_probs=ref_log_probs)
     if ratio not in ("step", "tour") or average not in (None, "step", "tour"):
