@@ -36,16 +36,32 @@ struct PolicyParams {
     float *loss, *stats;    // stats: kl, clip fraction
     double* partial;        // [blocks][4]; with one block unused
     double* norm;           // 1 / what the averages divide by
-    float2* rows;           // (T): gradient of the ratio term w.r.t. a whole tour's x; 1 / kept steps
+    double2* rows;          // (T): gradient of the ratio term w.r.t. a whole tour's x; 1 / kept steps
     const float* g;
     void* grad;
 };
 
+// Terms are computed as float, and where that gives no finite number again as double: a term past the range of float
+// may be in an average inside that range, and an advantage of 0 makes its own 0.  (All terms as double: 10000 x 1000
+// steps 39 + 33 -> 42 + 35 us.)
+// e^x as double: float's exponential, above 80 times e^80.  inf above 168, where no average of 2^62 steps is finite.
+template <typename F>
+__device__ __forceinline__ F exp_as(double x)
+{
+    if constexpr (sizeof(F) == 4) return expf((float)x);
+    const bool far = x > 80.0;
+    const double e = (double)expf((float)(far ? x - 80.0 : x));
+    return (F)(far ? e * 5.54062238439351e34 : e);
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
 // exp(d) - 1 - d.  Near 0 it is about d^2 / 2 and the subtraction would lose it: the series (to d^11, 2e-9 of the
 // result at |d| = 1) instead.
-__device__ __forceinline__ float kl_term(float d)
+template <typename F>
+__device__ __forceinline__ F kl_term(float d)
 {
-    if (fabsf(d) > 1.0f) return (expf(d) - 1.0f) - d;
+    if (fabsf(d) > 1.0f) return (exp_as<F>((double)d) - (F)1) - (F)d;
     float s = 1.0f / 11.0f;
     s = fmaf(s * d, 0.1f, 0.1f);
     s = fmaf(s * d, 1.0f / 9.0f, 1.0f / 9.0f);
@@ -56,7 +72,7 @@ __device__ __forceinline__ float kl_term(float d)
     s = fmaf(s * d, 1.0f / 4.0f, 1.0f / 4.0f);
     s = fmaf(s * d, 1.0f / 3.0f, 1.0f / 3.0f);
     s = fmaf(s * d, 1.0f / 2.0f, 1.0f / 2.0f);
-    return s * d * d;
+    return (F)(s * d * d);
 }
 
 // The ratio term of one step or tour.  The gradient jumps where the ratio leaves [lo, hi]; the side is decided on x in
@@ -66,11 +82,13 @@ __device__ __forceinline__ bool is_cut(const PolicyParams& p, float adv, double 
     return (adv > 0.0f && x > p.log_hi) || (adv < 0.0f && x < p.log_lo);
 }
 
-// -adv e^x where it is not cut.  An advantage of 0 makes it 0 also where e^x is past the range of float, which would give
-// 0 times inf; the steps of a long tour sum up to such an x.
-__device__ __forceinline__ float ratio_term(float adv, double x)
+// -adv e^x where it is not cut; 0 for an advantage of 0 and any x below inf (the steps of a long tour sum up to an e^x
+// past every range, which would give 0 times inf).
+template <typename F>
+__device__ __forceinline__ F ratio_term(float adv, double x)
 {
-    return adv == 0.0f && x < __builtin_inf() ? 0.0f : -adv * expf((float)x);
+    if (sizeof(F) == 8 && adv == 0.0f && x < __builtin_inf()) return (F)0;
+    return -(F)adv * exp_as<F>(x);
 }
 
 // Sum over a group of G threads (over the workgroup where G is more than a wave), in every thread of it.
@@ -153,6 +171,26 @@ __device__ __forceinline__ void policy_end(const PolicyParams& p, const double (
     p.stats[1] = (float)(v[2] * inv);
 }
 
+__device__ __forceinline__ float cut_term(const PolicyParams& p, float adv) { return -adv * (adv > 0.0f ? p.hi : p.lo); }
+
+// A thread's sums of a row again, of terms as double.
+template <typename E, int G>
+__device__ void far_sums(const PolicyParams& p, int64_t k, int at, float of_tour, double& ratio, double& kl)
+{
+    ratio = kl = 0.0;
+    for (int64_t s = at; s < p.S; s += G) {
+        const int64_t i = k * p.S + s;
+        if (p.mask && !p.mask[i]) continue;
+        const float lp = widen(static_cast<const E*>(p.lp)[i]);
+        if (!(p.mode & kRatioTour)) {
+            const float adv = p.adv_per_step ? p.adv[i] : of_tour;
+            const double x = (double)lp - (double)widen(static_cast<const E*>(p.old)[i]);
+            ratio += is_cut(p, adv, x) ? (double)cut_term(p, adv) : ratio_term<double>(adv, x);
+        }
+        if (p.ref) kl += kl_term<double>(widen(static_cast<const E*>(p.ref)[i]) - lp);
+    }
+}
+
 template <typename E, int G>
 __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
 {
@@ -180,12 +218,13 @@ __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
                     v[4] += x;
                 } else {
                     const bool cut = is_cut(p, adv[u], x);
-                    v[0] += (double)(cut ? -adv[u] * (adv[u] > 0.0f ? p.hi : p.lo) : ratio_term(adv[u], x));
+                    v[0] += (double)(cut ? cut_term(p, adv[u]) : ratio_term<float>(adv[u], x));
                     v[2] += cut ? 1.0 : 0.0;
                 }
-                if (p.ref) v[1] += (double)kl_term(ref[u] - lp[u]);
+                if (p.ref) v[1] += (double)kl_term<float>(ref[u] - lp[u]);
             }
         });
+        if (!(fabs(v[0]) < __builtin_inf() && v[1] < __builtin_inf())) far_sums<E, G>(p, k, g.at, of_tour, v[0], v[1]);
         if (p.mode == 0) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) sum[c] += v[c];
@@ -193,12 +232,12 @@ __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
         }
         group_sum<G>(v);
         const double inv = v[3] > 0.0 ? 1.0 / v[3] : 0.0;
-        float c = 0.0f;
+        double c = 0.0;
         if (p.mode & kRatioTour) {
             const float adv = p.adv[k];
             const bool cut = is_cut(p, adv, v[4]);
-            c = cut ? 0.0f : ratio_term(adv, v[4]);
-            v[0] = cut ? -adv * (adv > 0.0f ? p.hi : p.lo) : c;
+            c = cut ? 0.0 : ratio_term<double>(adv, v[4]);
+            v[0] = cut ? (double)cut_term(p, adv) : c;
             v[2] = cut ? 1.0 : 0.0;
         } else {
             v[0] *= inv;
@@ -206,7 +245,7 @@ __global__ __launch_bounds__(1024) void k_policy(PolicyParams p)
         }
         if (g.at == 0) {
             if (v[3] > 0.0) { sum[0] += v[0]; sum[1] += v[1] * inv; sum[2] += v[2]; sum[3] += 1.0; }
-            p.rows[k] = make_float2(v[3] > 0.0 ? c : 0.0f, (float)inv);
+            p.rows[k] = make_double2(v[3] > 0.0 ? c : 0.0, inv);
         }
     }
     group_sum<1024>(sum);
@@ -226,13 +265,31 @@ __global__ __launch_bounds__(1024) void k_policy_end(PolicyParams p, int blocks)
     if (threadIdx.x == 0) policy_end(p, v);
 }
 
+template <typename F>
+__device__ __forceinline__ F step_grad(const PolicyParams& p, const double2& row, double scale, float lp, float old,
+                                       float ref, float adv)
+{
+    F d;
+    if (p.mode & kRatioTour) {
+        d = (F)row.x;
+    } else {
+        const double x = (double)lp - (double)old;
+        d = is_cut(p, adv, x) ? (F)0 : ratio_term<F>(adv, x) * (F)row.y;
+    }
+    if (p.ref && p.kl_coef != 0.0) {
+        const float e = ref - lp;
+        d -= (F)p.kl_coef * (F)row.y * (fabsf(e) > 1.0f ? exp_as<F>((double)e) - (F)1 : kl_term<F>(e) + (F)e);
+    }
+    return d * (F)scale;
+}
+
 template <typename E, int G>
 __global__ __launch_bounds__(1024) void k_policy_grad(PolicyParams p)
 {
     const Groups<G> g;
-    const float scale = (float)(p.norm[0] * (double)p.g[0]);
+    const double scale = p.norm[0] * (double)p.g[0];
     for (int64_t k = g.first; k < p.T; k += g.count) {
-        const float2 row = p.mode ? p.rows[k] : make_float2(0.0f, 1.0f);
+        const double2 row = p.mode ? p.rows[k] : make_double2(0.0, 1.0);
         const float of_tour = p.adv_per_step ? 0.0f : p.adv[k];
         for_steps<G>(g.at, p.S, [&](auto many, int64_t first) {
             constexpr int N = decltype(many)::value;
@@ -248,17 +305,8 @@ __global__ __launch_bounds__(1024) void k_policy_grad(PolicyParams p)
             for (int u = 0; u < N; ++u) {
                 float d = 0.0f;
                 if (kept[u]) {
-                    if (p.mode & kRatioTour) {
-                        d = row.x;
-                    } else {
-                        const double x = (double)lp[u] - (double)old[u];
-                        d = is_cut(p, adv[u], x) ? 0.0f : ratio_term(adv[u], x) * row.y;
-                    }
-                    if (p.ref && p.kl_coef != 0.0) {
-                        const float e = ref[u] - lp[u];
-                        d -= (float)p.kl_coef * row.y * (fabsf(e) > 1.0f ? expf(e) - 1.0f : kl_term(e) + e);
-                    }
-                    d *= scale;
+                    d = step_grad<float>(p, row, scale, lp[u], old[u], ref[u], adv[u]);
+                    if (!finite(d)) d = (float)step_grad<double>(p, row, scale, lp[u], old[u], ref[u], adv[u]);
                 }
                 static_cast<E*>(p.grad)[i + u * G] = narrow<E>(d);
             }
@@ -458,7 +506,7 @@ Shape shape_of(int64_t T, int64_t S, bool one_block)
         default: { constexpr int G = kBlockRow; CALL; break; }     \
     }
 
-int64_t policy_state_bytes(int64_t T) { return kPartialBytes + round256(8 * T); }
+int64_t policy_state_bytes(int64_t T) { return kPartialBytes + round256(16 * T); }
 
 int64_t pref_state_bytes(int64_t T) { return kPartialBytes + round256(8 * T) + 2 * round256(4 * T); }
 
@@ -479,7 +527,7 @@ void policy_state(PolicyParams& p, void* state)
     char* at = static_cast<char*>(state);
     p.norm = reinterpret_cast<double*>(at);
     p.partial = reinterpret_cast<double*>(at + 256);
-    p.rows = reinterpret_cast<float2*>(at + kPartialBytes);
+    p.rows = reinterpret_cast<double2*>(at + kPartialBytes);
 }
 
 int policy_fill(PolicyParams& p, const void* lp, const void* old, const void* ref, const float* adv,

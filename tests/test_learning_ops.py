@@ -693,6 +693,39 @@ def test_gpu_policy_loss_of_zero_advantages_and_far_ratios(ratio, average, per_s
 
 
 @gpu
+@pytest.mark.parametrize("ratio,average,per_step", [("step", "step", False), ("step", "step", True), ("step", "tour", False),
+                                                    ("tour", "tour", False)])
+@pytest.mark.parametrize("T,S", [(200, 50), (3, 5000)])
+def test_gpu_policy_loss_of_terms_past_the_range_of_float(T, S, ratio, average, per_step):
+    """Single terms above 3.4e38 in averages below it: sums are in double, so are such terms.  e^95 carries the rounding
+    of its argument, 95 u, the exponential's own 2 ulp and a handful of products: below 8 u (4 + 95) of it."""
+    import ml4tspbench_amd as amd
+    gen = torch.Generator().manual_seed(18)
+    lp = -torch.rand((T, S), generator=gen) - 0.5
+    old = lp - 0.01 * torch.randn((T, S), generator=gen) / math.sqrt(S)
+    ref = lp + 0.3 * torch.randn((T, S), generator=gen)
+    adv = torch.randn(T, generator=gen)
+    adv[1:] = -adv[1:].abs()                # where the ratio may grow
+    far = 95.0 if average == "step" else 89.5           # averages of tours divide by less
+    old[1, 3] -= far
+    ref[T - 1, S // 2] += far               # another tour: the gradient's parts do not cancel
+    lp[2, 0] += 60.0                        # far, and within the range
+    adv_in = adv[:, None].expand(T, S).contiguous() if per_step else adv
+    x = lp.cuda().requires_grad_()
+    coef = 0.1 if average == "step" else 0.01
+    res = amd.clipped_policy_loss(x, old.cuda(), adv_in.cuda(), ref_log_probs=ref.cuda(), kl_coef=coef, ratio=ratio,
+                                  average=average)
+    (dx,) = torch.autograd.grad(res.loss, x, torch.tensor(0.001, device="cuda"))
+    loss, kl, clip, grad, size = ref_policy(lp, old, adv_in, ref, None, 0.2, 0.2, coef, ratio, average)
+    share = 8 * U * (4 + 95)
+    for name, got, want in (("loss", res.loss, loss), ("kl", res.kl, kl), ("gradient", dx, 0.001 * grad)):
+        ok = want.abs() <= torch.finfo(torch.float32).max           # a result past it is inf
+        assert torch.equal(got.detach().isfinite().cpu(), ok), name
+        compare(name, got.detach().cpu()[ok], want[ok], share * want.abs()[ok] + share * 0.001 * coef)
+    assert float(loss) > 1e30
+
+
+@gpu
 def test_gpu_policy_loss_small_kl_keeps_its_digits():
     """d of 1e-4: exp(d) - 1 - d is 5e-9, of which float32 subtraction would leave nothing."""
     import ml4tspbench_amd as amd
