@@ -301,15 +301,19 @@ __global__ __launch_bounds__(1024) void k_policy_grad(PolicyParams p)
             load_steps<E, N, G>(p.ref, i, p.ref && p.kl_coef != 0.0, 0.0f, ref);
             load_steps<float, N, G>(p.adv, i, p.adv_per_step, of_tour, adv);
             load_kept<N, G>(p.mask, i, kept);
+            float d[N], all = 0.0f;
 #pragma unroll
             for (int u = 0; u < N; ++u) {
-                float d = 0.0f;
-                if (kept[u]) {
-                    d = step_grad<float>(p, row, scale, lp[u], old[u], ref[u], adv[u]);
-                    if (!finite(d)) d = (float)step_grad<double>(p, row, scale, lp[u], old[u], ref[u], adv[u]);
-                }
-                static_cast<E*>(p.grad)[i + u * G] = narrow<E>(d);
+                d[u] = kept[u] ? step_grad<float>(p, row, scale, lp[u], old[u], ref[u], adv[u]) : 0.0f;
+                all += d[u];
             }
+            if (!finite(all)) {
+#pragma unroll
+                for (int u = 0; u < N; ++u)
+                    if (!finite(d[u])) d[u] = (float)step_grad<double>(p, row, scale, lp[u], old[u], ref[u], adv[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < N; ++u) static_cast<E*>(p.grad)[i + u * G] = narrow<E>(d[u]);
         });
     }
 }
