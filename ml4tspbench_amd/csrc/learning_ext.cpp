@@ -87,7 +87,9 @@ Tensor state_like(const Tensor& x, int64_t bytes) { return at::empty({bytes}, x.
 Tensor once(Tensor grad, const variable_list& incoming)
 {
     if (!c10::GradMode::is_enabled()) return grad;
-    auto edges = torch::autograd::get_current_node()->next_edges();
+    const auto self = torch::autograd::get_current_node();
+    TORCH_CHECK(self, "the learning operators' gradient is taken with create_graph outside of autograd's engine");
+    auto edges = self->next_edges();
     for (auto& edge : torch::autograd::collect_next_edges(incoming)) edges.push_back(std::move(edge));
     torch::autograd::set_history(grad, std::make_shared<torch::autograd::Error>(
                                            "the learning operators have no second derivative", std::move(edges)));
